@@ -548,3 +548,30 @@ def test_chain_of_layers(M):
         graph.replay()
         assert torch.equal(got, want)
     check_status()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("M,N,off", [(3, 264, 8), (140, 136, 3), (1500, 1672, 8), (1500, 1672, 3)])
+def test_activations_of_the_largest_arguments(fmt, dtype, activation, M, N, off):
+    """Arguments whose square passes the range of 32 bits, infinities and NaN, in both kernels' epilogues: what the formula gives.  All but
+    the first 32 columns are finite, so the blocks behind them are too."""
+    a, w = stored(M, 64, fmt, M), stored(N, 64, fmt, N)
+    a.tensor_scale = 2.0 ** -7
+    large = torch.tensor([1e20, -1e20, 3e38, -3e38, 2e19, -2e19, 1.8e19, -1.8e19, 5.0, -5.0, 0.0, 1e30, -1e30, 1e10, -1e10, -80.0, 90.0])
+    bias = large[torch.arange(N) % len(large)]
+    bias[:4] = torch.tensor([math.inf, -math.inf, math.nan, 1e20])
+    wide = torch.empty(M, N + 16, dtype=dtype, device=DEV)
+    kw = dict(bias=bias.to(DEV), activation=activation)
+    got = fp4_matmul(a, w, out=wide[:, off:off + N], **kw).cpu().double()
+    want, size = plain64.matmul(values(a), values(w), bias=bias, activation=activation)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    assert bool((got[:, 0] == math.inf).all()) and bool(want[:, 3:].isfinite().all())
+    err = (got - want).abs()[:, 3:]
+    assert bool((err <= ULP[dtype] * want[:, 3:].abs() + 80 * 2.0 ** -23 * size[:, 3:]).all())
+    quantised = fp4_matmul(a, w, dtype=fmt, **kw)
+    for x, y in zip(codes_of(quantised), codes_of(fp4_quantize(fp4_matmul(a, w, dtype=F32, **kw), fmt))):
+        assert torch.equal(x, y)
+    assert bool(values(quantised)[:, 32:].isfinite().all())
+    check_status()

@@ -109,19 +109,22 @@ __device__ __forceinline__ void tma_load_tile3_pair(uint32_t dst, const void* ma
 
 // ---- epilogue ---------------------------------------------------------------------
 // tanh(u) = 2 / (1 + exp(-2 u)) - 1, so both activations are x / (1 + 2^-z).  ex2 and rcp are good to 2^-22; z, of a few
-// tens at most where the result is not x or 0, adds 2^-20 at worst.
+// tens at most where the result is not x or 0, adds 2^-20 at worst.  Large arguments: z overflows to an infinity of the right sign
+// and the result is x or -0.  GELU's x^2 may overflow in it; SiLU has no such term (times a factor of 0 it would be a NaN).
 template <int n>
 __device__ __forceinline__ void mm_act(float (&y)[n], int act) {
   if (act == T2T_ACT_NONE) return;
   constexpr float log2e = 1.4426950408889634f;
   const float c1 = act == T2T_ACT_SILU ? -log2e : -1.5957691216057308f * log2e;
-  const float c3 = act == T2T_ACT_SILU ? 0.f : 0.044715f * -1.5957691216057308f * log2e;
+  constexpr float c3 = 0.044715f * -1.5957691216057308f * log2e;
   const uint64_t k1 = pair_of(c1, c1), k3 = pair_of(c3, c3), one = pair_of(1.f, 1.f);
 #pragma unroll
   for (int e = 0; e < n; e += 2) {
     const uint64_t x = pair_of(y[e], y[e + 1]);
     float p, q;
-    pair_to(mul2(x, fma2(k3, mul2(x, x), k1)), p, q);
+    uint64_t z = k1;
+    if (act == T2T_ACT_GELU_TANH) z = fma2(k3, mul2(x, x), k1);
+    pair_to(mul2(x, z), p, q);
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(q));
     pair_to(add2(pair_of(p, q), one), p, q);
