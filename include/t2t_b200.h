@@ -282,6 +282,14 @@ int t2t_softmax_give_up_selftest(int commits, unsigned handed, void* out, float*
  * unless nothing is missing.  The kernel always terminates.  No counterpart in the reference. */
 int t2t_select_give_up_selftest(int stuck, int* d_left, int* d_status, cudaStream_t stream);
 
+/* Give-up paths of the 4-bit products: residual + A W^T of T2T_NVFP4 matrices A [M, K], W [N, K] (tensor scales 1), residual and out
+ * [M, N] bf16 with contiguous rows, 16-byte aligned, N a multiple of 8; up to 16 rows, or so many that the product takes pairs of
+ * CTAs.  `stuck`: 1 has the kernel wait for 16 bytes more of the first operands than there are, 2 (pairs of CTAs) of the residuals
+ * of every CTA's last tile.  The waits run out within milliseconds, *d_status becomes 1 (wait timed out), what depends on them is
+ * not written.  0: nothing is missing.  The kernel always terminates.  No counterpart in the reference. */
+int t2t_fp4_give_up_selftest(int stuck, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
+                             int M, int N, int K, const void* residual, void* out, int* d_status, cudaStream_t stream);
+
 /* What the attention entry points check of their two kernels before the first launch on a device, for a
  * kernel built with `regs` registers a thread: 0 if the split of registers between its warps holds,
  * T2T_ERR_CUDA otherwise (its warps would wait for registers that do not exist).  Host only.  No counterpart

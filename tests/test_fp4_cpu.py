@@ -80,3 +80,14 @@ def test_tensor_scale():
 def test_few_rows():
     header = (pathlib.Path(__file__).parents[1] / "include" / "t2t_b200.h").read_text()
     assert f"#define T2T_FP4_FEW_ROWS {FEW_ROWS}\n" in header
+
+
+def test_give_up_selftest_refuses_bad_arguments(lib):
+    x = 4096                     # never read
+
+    def call(stuck=1, a=x, M=4, N=8, K=64, residual=x, out=x, status=x):
+        return lib.t2t_fp4_give_up_selftest(stuck, a, x, x, x, M, N, K, residual, out, status, 0)
+
+    for kw in (dict(stuck=-1), dict(stuck=3), dict(a=0), dict(a=x + 8), dict(M=0), dict(N=0), dict(N=9), dict(K=0), dict(residual=0), dict(out=0),
+               dict(out=x + 2), dict(status=0)):
+        assert call(**kw) == 1, kw

@@ -575,3 +575,50 @@ def test_activations_of_the_largest_arguments(fmt, dtype, activation, M, N, off)
         assert torch.equal(x, y)
     assert bool(values(quantised)[:, 32:].isfinite().all())
     check_status()
+
+
+@pytest.mark.parametrize("stuck,M,N,K", [(1, 1, 512, 2048), (1, 16, 40, 96), (1, 1500, 1672, 96), (1, 1500, 1672, 2080),
+                                         (2, 1500, 1672, 96), (2, 3000, 5120, 96)])
+def test_product_that_gave_up_says_so(lib, stuck, M, N, K):
+    """Bytes that never come, of the first operands or of the last residuals: the waits run out, every CTA ends, the status says so, and the
+    next product is as before.  Run with nothing missing in between."""
+    a, w = stored(M, K, "nvfp4", 1), stored(N, K, "nvfp4", 2)
+    residual = torch.randn(M, N, generator=gen(3)).to(BF).to(DEV)
+    want = fp4_matmul(a, w, residual=residual)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(want)
+
+    def run(stuck):
+        status.zero_()
+        out.copy_(residual).mul_(0).sub_(7)
+        code = lib.t2t_fp4_give_up_selftest(stuck, *a.pointers(), *w.pointers(), M, N, K, residual.data_ptr(), out.data_ptr(),
+                                            status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert code == 0
+        return int(status.item())
+
+    for _ in range(3):
+        assert run(0) == 0 and torch.equal(out, want)
+        assert run(stuck) == 1
+        same = out == want
+        assert not bool(same.all())
+        if stuck == 2:      # only what lies behind the last residuals is missing
+            assert bool((same | (out == -7)).all()) and bool(same.any())
+    assert torch.equal(fp4_matmul(a, w, residual=residual), want)
+    check_status()
+
+
+def test_status_of_an_earlier_product_is_raised_once():
+    """A product that gave up writes to its device's word; whatever is called next says so, and works from then on."""
+    from token2tile_b200.fp4 import _status_of
+    x = torch.randn(5, 64, generator=gen(1)).to(BF).to(DEV)
+    layer = Fp4Linear(torch.randn(32, 64, generator=gen(2)).to(BF).to(DEV))
+    back = Fp4Linear(torch.randn(64, 32, generator=gen(3)).to(BF).to(DEV))
+    a = fp4_quantize(x)
+    for call in (lambda: fp4_matmul(a, layer.w), lambda: fp4_matmul(a, layer.w, dtype="nvfp4"), lambda: layer(x), lambda: layer(x[:1]),
+                 lambda: layer(a), lambda: Fp4FeedForward(layer, back)(x), check_status, lambda: check_status(wait=False)):
+        call()
+        _status_of(x.device).value.value = 1
+        with pytest.raises(RuntimeError, match="fp4_matmul"):
+            call()
+        call()
+    check_status()

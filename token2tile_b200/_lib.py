@@ -56,6 +56,7 @@ SIGNATURES = {
     "t2t_wait_timeout_selftest": (_I, [_P, _P, _P]),
     "t2t_softmax_give_up_selftest": (_I, [_I, C.c_uint, _P, _P, _P, _P, _P]),
     "t2t_select_give_up_selftest": (_I, [_I, _P, _P, _P]),
+    "t2t_fp4_give_up_selftest": (_I, [_I] + [_P] * 4 + [_I] * 3 + [_P] * 4),
     "t2t_register_split_selftest": (_I, [_I]),
     "t2t_rotary": (_I, [_P] * 6 + [_I, _P, _I, _L, _L, _P, _P, _P] + [_I] * 9 + [_F, _F, _I, _P]),
     "t2t_rotary_grad_ws_bytes": (_S, [_I, _I, _I, _I]),

@@ -41,7 +41,15 @@ struct MmArgs {
   long long x_row;
   int x_dtype;
   bool x_wide;              // its rows are 16-byte aligned
+  int stuck;                // give-up self-test: what never arrives
 };
+// 1: bytes of the first operands; 2: bytes of the residuals of every CTA's last tile.
+enum { MM_STUCK_NONE, MM_STUCK_OPERANDS, MM_STUCK_RESIDUAL };
+// Limit of the waits: the self-test's run out within milliseconds.
+template <bool GIVE_UP>
+__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_wait_warp(bar, parity, abort_flag, GIVE_UP ? 1u << 12 : kWaitSpinLimit);
+}
 
 constexpr int MM_TILE = 256;                       // rows and columns of a pair's tile
 constexpr int MM_K = 256;                          // codes of K a stage: 128 bytes a row
@@ -284,7 +292,17 @@ __device__ __forceinline__ void mm_tile(int tile, int mt, int nt, int& m0, int& 
   n0 = at / rows * MM_TILE;
 }
 
-template <int FMT, typename T, MmEpilogue EPI>
+// Behind a barrier of the CTA after its last wait: reports one that gave up, and lets copies still in flight land before the shared memory
+// is released.
+__device__ __forceinline__ void mm_gave_up(const MmArgs& p, volatile int* abort_flag) {
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && p.status) *reinterpret_cast<volatile int*>(p.status) = ST_WAIT_TIMEOUT;
+    for (int i = 0; i < 100; ++i) __nanosleep(1000);
+  }
+  __syncwarp();
+}
+
+template <int FMT, typename T, MmEpilogue EPI, bool GIVE_UP = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
     fp4_mm_pair_kernel(const __grid_constant__ MmMaps maps, const MmArgs p) {
   extern __shared__ uint8_t smem_raw[];
@@ -332,11 +350,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
       mm_tile(tile, mt, nt, m0, n0);
       for (int k = 0; k < steps; ++k, ++it) {
         const uint32_t s = it % MM_STAGES;
-        ok = it < MM_STAGES || mbar_wait_warp(bars + MB_EMPTY + s, (it / MM_STAGES - 1u) & 1u, abort_flag);
+        ok = it < MM_STAGES || mm_wait<GIVE_UP>(bars + MB_EMPTY + s, (it / MM_STAGES - 1u) & 1u, abort_flag);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t full = lead + (MB_FULL + s) * 8, codes = base + s * 2 * MM_HALF, sc = s_scales + s * 3 * ATOMS * 512;
-          if (rank == 0) mbar_arrive_expect_tx(bars + MB_FULL + s, 2 * STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(bars + MB_FULL + s, 2 * STAGE + (GIVE_UP && p.stuck == MM_STUCK_OPERANDS && it == 0 ? 16 : 0));
           tma_load_tile_pair(codes, &maps.a, k * 128, m0 + (int)rank * 128, full);
           tma_load_tile_pair(codes + MM_HALF, &maps.w, k * 128, n0 + (int)rank * 128, full);
           tma_load_tile3_pair(sc, &maps.sa, 0, k * ATOMS, m0 / 128 + (int)rank, full);
@@ -347,7 +365,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
     }
     // the products that read the last stages have arrived here too before this CTA leaves
     for (uint32_t i = it < MM_STAGES ? 0 : it - MM_STAGES; ok && i < it; ++i)
-      ok = mbar_wait_warp(bars + MB_EMPTY + i % MM_STAGES, (i / MM_STAGES) & 1u, abort_flag);
+      ok = mm_wait<GIVE_UP>(bars + MB_EMPTY + i % MM_STAGES, (i / MM_STAGES) & 1u, abort_flag);
   } else if (warp == 1 && rank == 0) {
     // ================= products =================
     constexpr uint32_t dhi = sdesc_hi(1024);
@@ -355,12 +373,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
     bool ok = true;
     for (int tile = first; tile < tiles; tile += stride, ++n) {
       // the epilogue has read the columns that this tile shares with the one before (and all of the one before that)
-      if (n > 0 && !mbar_wait_warp(bars + MB_DRAINED, (n - 1u) & 1u, abort_flag)) break;
+      if (n > 0 && !mm_wait<GIVE_UP>(bars + MB_DRAINED, (n - 1u) & 1u, abort_flag)) break;
       tc_fence_after();
       const uint32_t acc = tmem + (n & 1u) * MM_ACC1;
       for (int k = 0; k < steps; ++k, ++it) {
         const uint32_t s = it % MM_STAGES;
-        ok = mbar_wait_warp(bars + MB_FULL + s, (it / MM_STAGES) & 1u, abort_flag);
+        ok = mm_wait<GIVE_UP>(bars + MB_FULL + s, (it / MM_STAGES) & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -401,7 +419,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
       const bool odd = n & 1u;
       const uint32_t acc = tmem_addr(tmem + (n & 1u) * MM_ACC1, quad * 32, 0);
       auto wait_acc = [&] {
-        ok = ok && mbar_wait_warp(bars + MB_ACC + (n & 1u), (n >> 1) & 1u, abort_flag);
+        ok = ok && mm_wait<GIVE_UP>(bars + MB_ACC + (n & 1u), (n >> 1) & 1u, abort_flag);
         tc_fence_after();
       };
       auto drained = [&] {
@@ -434,7 +452,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
           if (row == 0) {
             tma_store_wait<true>();      // the tile before has left the buffer
             if (p.residual && there && ok) {
-              mbar_arrive_expect_tx(bars + MB_RES + group, 16384);
+              const bool stuck = GIVE_UP && p.stuck == MM_STUCK_RESIDUAL && tile + stride >= tiles && i + 1 == PER;
+              mbar_arrive_expect_tx(bars + MB_RES + group, 16384 + (stuck ? 16 : 0));
               tma_load_tile(smem_u32(buffer), &maps.res, col, rows0, bars + MB_RES + group);
             }
           }
@@ -449,7 +468,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
           if (i == 0) drained();
           mm_meet(group);
           if (p.residual && there) {
-            ok = ok && mbar_wait_warp(bars + MB_RES + group, loads & 1u, abort_flag);
+            ok = ok && mm_wait<GIVE_UP>(bars + MB_RES + group, loads & 1u, abort_flag);
             ++loads;
           }
           if (ok && there) {
@@ -502,13 +521,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mm_threads(EPI), 1)
     if (EPI == MM_TMA && row == 0) tma_store_wait<false>();
   }
   __syncwarp();
-  if (*abort_flag) {
-    if (tid == 0 && p.status) *reinterpret_cast<volatile int*>(p.status) = ST_WAIT_TIMEOUT;
-    // a wait gave up: let copies still in flight land before the shared memory is released
-    for (int i = 0; i < 100; ++i) __nanosleep(1000);
-  }
   tc_fence_before();
-  __syncthreads();
+  __syncthreads();      // every wait of the CTA has ended, those for the last residuals too
+  mm_gave_up(p, abort_flag);
   cluster_sync();      // the other CTA no longer arrives here, and both are done with tensor memory
   if (warp == 0) tmem_dealloc_pair(tmem, 512);
 }
@@ -616,7 +631,7 @@ __device__ __forceinline__ void mr_finish(const MmArgs& p, int m, int n, float (
 // 16 elements to a lane.  The codes and scales are those of the quantisation on its own.  They run beside the
 // copies of W: 4 x 5,120 x 5,120 nvfp4 takes 5.9 us like this, 6.0 from codes and 7.7 with the quantisation as a launch of its own (one
 // row 5.7, 6.2 and 7.3).  Sixteen rows fell behind the products (11.6 us, 8.8 in two launches).
-template <int FMT, int STAGES, typename X>
+template <int FMT, int STAGES, typename X, bool GIVE_UP>
 __device__ __forceinline__ void mr_quantize(const MmArgs& p, int w, int first, int last, uint8_t* codes, int codes_stage, uint8_t* scales,
                                             int scales_stage, uint64_t* full, uint64_t* empty, volatile int* abort_flag) {
   constexpr int B = fp4_block(FMT), ATOMS = mm_stage_atoms(FMT), UNITS = MM_K / 16, ROWS = 32 / UNITS, LOOKS = T2T_FP4_FEW_ROWS / ROWS;
@@ -633,7 +648,7 @@ __device__ __forceinline__ void mr_quantize(const MmArgs& p, int w, int first, i
       if (p.x_wide) load_raw<X, true>(q, left, raw[j]);
       else load_raw<X, false>(q, left, raw[j]);
     }
-    if (it >= STAGES && !mbar_wait_warp(empty + s, (it / STAGES - 1u) & 1u, abort_flag)) return;
+    if (it >= STAGES && !mm_wait<GIVE_UP>(empty + s, (it / STAGES - 1u) & 1u, abort_flag)) return;
 #pragma unroll
     for (int j = 0; j < LOOKS; ++j) {
       if (j * ROWS >= p.M) break;
@@ -658,7 +673,7 @@ __device__ __forceinline__ void mr_quantize(const MmArgs& p, int w, int first, i
 
 // Grid: (splits x slabs of 128 rows of W, tiles of T rows of A); clusters of `splits` CTAs.  X: void, or the type of an A that is quantised
 // here (one tile of rows).
-template <int FMT, int T, typename OUT, typename X>
+template <int FMT, int T, typename OUT, typename X, bool GIVE_UP = false>
 __global__ void __launch_bounds__(MR_THREADS) fp4_mm_rows_kernel(const __grid_constant__ MmMaps maps, const MmArgs p, int splits) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int STAGES = mr_stages(T), STAGE = mr_stage_bytes(FMT, T), ATOMS = mm_stage_atoms(FMT), COLUMNS = mr_columns(T);
@@ -692,11 +707,12 @@ __global__ void __launch_bounds__(MR_THREADS) fp4_mm_rows_kernel(const __grid_co
   if (warp == 0) {
     for (int k = first; k < last; ++k) {
       const uint32_t it = k - first, s = it % STAGES;
-      if (it >= STAGES && !mbar_wait_warp(bars + STAGES + s, (it / STAGES - 1u) & 1u, abort_flag)) break;
+      if (it >= STAGES && !mm_wait<GIVE_UP>(bars + STAGES + s, (it / STAGES - 1u) & 1u, abort_flag)) break;
       if (elect_one()) {
         uint64_t* full = bars + s;
         const uint32_t sc = s_scales + s * 2 * ATOMS * 512;
-        mbar_arrive_expect_tx(full, QUANTIZE ? MM_HALF + ATOMS * 512 : STAGE);
+        const int stuck = GIVE_UP && p.stuck == MM_STUCK_OPERANDS && it == 0 ? 16 : 0;
+        mbar_arrive_expect_tx(full, (QUANTIZE ? MM_HALF + ATOMS * 512 : STAGE) + stuck);
         tma_load_tile(base + s * MM_HALF, &maps.w, k * 128, n0, full);
         tma_load_tile3(sc, &maps.sw, 0, k * ATOMS, n0 / 128, full);
         if (!QUANTIZE) {
@@ -710,7 +726,7 @@ __global__ void __launch_bounds__(MR_THREADS) fp4_mm_rows_kernel(const __grid_co
     constexpr uint32_t dhi = sdesc_hi(1024);
     for (int k = first; k < last; ++k) {
       const uint32_t it = k - first, s = it % STAGES;
-      if (!mbar_wait_warp(bars + s, (it / STAGES) & 1u, abort_flag)) break;
+      if (!mm_wait<GIVE_UP>(bars + s, (it / STAGES) & 1u, abort_flag)) break;
       tc_fence_after();
       if (elect_one()) {
         const uint32_t sc = s_scales + s * 2 * ATOMS * 512;
@@ -732,11 +748,11 @@ __global__ void __launch_bounds__(MR_THREADS) fp4_mm_rows_kernel(const __grid_co
       __syncwarp();
     }
   } else if constexpr (QUANTIZE) {
-    mr_quantize<FMT, STAGES, X>(p, warp - 2, first, last, sm + (s_rows - base), T * 128, sm + (s_scales - base) + ATOMS * 512,
+    mr_quantize<FMT, STAGES, X, GIVE_UP>(p, warp - 2, first, last, sm + (s_rows - base), T * 128, sm + (s_scales - base) + ATOMS * 512,
                                 2 * ATOMS * 512, bars, bars + STAGES, abort_flag);
   }
   // every warp waits for the sums: all copies have been read then, so that their memory is free (a rank without steps has none)
-  const bool any = last > first, ok = !any || mbar_wait_warp(bars + 2 * STAGES, 0, abort_flag);
+  const bool any = last > first, ok = !any || mm_wait<GIVE_UP>(bars + 2 * STAGES, 0, abort_flag);
   tc_fence_after();
   float* part = reinterpret_cast<float*>(sm);      // [T][128]
   if (warp >= 2 && ok) {
@@ -753,14 +769,10 @@ __global__ void __launch_bounds__(MR_THREADS) fp4_mm_rows_kernel(const __grid_co
     }
   }
   __syncwarp();
-  if (*abort_flag) {
-    if (tid == 0 && p.status) *reinterpret_cast<volatile int*>(p.status) = ST_WAIT_TIMEOUT;
-    // a wait gave up: let copies still in flight land before the shared memory is released
-    for (int i = 0; i < 100; ++i) __nanosleep(1000);
-  }
   tc_fence_before();
   if (splits > 1) cluster_sync();
   else __syncthreads();
+  mm_gave_up(p, abort_flag);
   if (warp == 0) tmem_dealloc(tmem, COLUMNS);
 
   const int n = n0 + lane * 4, rows = min(T, p.M - m0);
@@ -825,9 +837,9 @@ struct MmLaunch {
   }
 };
 
-template <int FMT, int T, typename OUT, typename X = void>
+template <int FMT, int T, typename OUT, typename X = void, bool GIVE_UP = false>
 static int mm_launch_rows(const MmMaps& maps, const MmArgs& p, int splits, cudaStream_t st) {
-  auto* k = fp4_mm_rows_kernel<FMT, T, OUT, X>;
+  auto* k = fp4_mm_rows_kernel<FMT, T, OUT, X, GIVE_UP>;
   constexpr int smem = mr_smem(FMT, T);
   static std::atomic<unsigned long long> allowed{0};
   if (!allow_smem(k, smem, allowed)) return T2T_ERR_CUDA;
@@ -835,9 +847,9 @@ static int mm_launch_rows(const MmMaps& maps, const MmArgs& p, int splits, cudaS
   return cudaLaunchKernelEx(&l.cfg, k, maps, p, splits) == cudaSuccess ? T2T_OK : T2T_ERR_CUDA;
 }
 
-template <int FMT, typename T, MmEpilogue EPI>
+template <int FMT, typename T, MmEpilogue EPI, bool GIVE_UP = false>
 static int mm_launch_pairs(const MmMaps& maps, const MmArgs& p, cudaStream_t st) {
-  auto* k = fp4_mm_pair_kernel<FMT, T, EPI>;
+  auto* k = fp4_mm_pair_kernel<FMT, T, EPI, GIVE_UP>;
   static std::atomic<unsigned long long> allowed{0};
   if (!allow_smem(k, mm_smem(FMT, EPI), allowed)) return T2T_ERR_CUDA;
   const long long tiles = (long long)cdiv(p.M, MM_TILE) * cdiv(p.N, MM_TILE);
@@ -845,6 +857,14 @@ static int mm_launch_pairs(const MmMaps& maps, const MmArgs& p, cudaStream_t st)
   if (pairs < 1) return T2T_ERR_CUDA;
   MmLaunch l(dim3(2 * pairs), mm_threads(EPI), mm_smem(FMT, EPI), 0, st);
   return cudaLaunchKernelEx(&l.cfg, k, maps, p) == cudaSuccess ? T2T_OK : T2T_ERR_CUDA;
+}
+
+template <typename T>
+static bool mm_result_maps(MmMaps& maps, const MmArgs& p) {
+  constexpr int size = sizeof(T);
+  constexpr bool half = std::is_same<T, __half>::value;
+  return make_result_map(&maps.out, p.out, size, half, p.N, p.M, p.out_row) &&
+         (!p.residual || make_result_map(&maps.res, p.residual, size, half, p.N, p.M, p.res_row));
 }
 
 template <int FMT, typename T>
@@ -866,11 +886,7 @@ static int mm_launch(MmMaps& maps, const MmArgs& p, const MmPlan& plan, cudaStre
     return mm_launch_pairs<FMT, T, MM_CODES>(maps, p, st);
   } else {
     if (!p.wide) return mm_launch_pairs<FMT, T, MM_LANES>(maps, p, st);
-    constexpr int size = sizeof(T);
-    constexpr bool half = std::is_same<T, __half>::value;
-    if (!make_result_map(&maps.out, p.out, size, half, p.N, p.M, p.out_row) ||
-        (p.residual && !make_result_map(&maps.res, p.residual, size, half, p.N, p.M, p.res_row)))
-      return T2T_ERR_CUDA;
+    if (!mm_result_maps<T>(maps, p)) return T2T_ERR_CUDA;
     return mm_launch_pairs<FMT, T, MM_TMA>(maps, p, st);
   }
 }
@@ -879,6 +895,14 @@ static int mm_launch(MmMaps& maps, const MmArgs& p, const MmPlan& plan, cudaStre
 
 using namespace t2t;
 
+static bool mm_operand_maps(MmMaps& maps, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, int fmt,
+                            const MmArgs& p, const MmPlan& plan) {
+  const int pitch = fp4_pitch(p.K), atoms = fp4_atoms(p.K, fmt), box = mm_stage_atoms(fmt);
+  return (p.x || (make_bytes_tile_map(&maps.a, a_codes, pitch, p.M, plan.T ? plan.T : 128) &&
+                  make_scale_map(&maps.sa, a_scales, atoms, cdiv(p.M, 128), box, 1))) &&
+         make_bytes_tile_map(&maps.w, w_codes, pitch, p.N, 128) &&
+         make_scale_map(&maps.sw, w_scales, atoms, cdiv(p.N, 128), box, plan.T ? 1 : 2);
+}
 // Checks and launch common to the two entry points; dtype < 0: quantised results.
 static int mm_run(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, int fmt, int dtype,
                   const MmArgs& p, cudaStream_t stream) {
@@ -890,12 +914,7 @@ static int mm_run(const void* a_codes, const void* a_scales, const void* w_codes
   if (sm_count() < 2) return T2T_ERR_CUDA;
   const MmPlan plan = mm_plan(p.M, p.N, p.K);
   MmMaps maps;
-  const int pitch = fp4_pitch(p.K), atoms = fp4_atoms(p.K, fmt), box = mm_stage_atoms(fmt);
-  if ((!p.x && (!make_bytes_tile_map(&maps.a, a_codes, pitch, p.M, plan.T ? plan.T : 128) ||
-                !make_scale_map(&maps.sa, a_scales, atoms, cdiv(p.M, 128), box, 1))) ||
-      !make_bytes_tile_map(&maps.w, w_codes, pitch, p.N, 128) ||
-      !make_scale_map(&maps.sw, w_scales, atoms, cdiv(p.N, 128), box, plan.T ? 1 : 2))
-    return T2T_ERR_CUDA;
+  if (!mm_operand_maps(maps, a_codes, a_scales, w_codes, w_scales, fmt, p, plan)) return T2T_ERR_CUDA;
 #define T2T_CALL(T) return fmt == T2T_MXFP4 ? mm_launch<T2T_MXFP4, T>(maps, p, plan, stream) : mm_launch<T2T_NVFP4, T>(maps, p, plan, stream)
   if (dtype < 0) T2T_CALL(uint8_t);
   if (dtype == T2T_BF16) T2T_CALL(__nv_bfloat16);
@@ -1001,4 +1020,31 @@ extern "C" int t2t_fp4_feed_forward(const void* x, long long x_row_stride, const
   if (rc != T2T_OK) return rc;
   return t2t_fp4_matmul(h, hs, down_codes, down_scales, M, N, F, fmt, down_scale, down_bias, T2T_ACT_NONE, gate, down_vec_dtype,
                         residual, residual_row_stride, out, out_row_stride, dtype, d_status, stream);
+}
+
+extern "C" int t2t_fp4_give_up_selftest(int stuck, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
+                                        int M, int N, int K, const void* residual, void* out, int* d_status, cudaStream_t stream) {
+  if (!a_codes || !a_scales || !w_codes || !w_scales || !residual || !out || !d_status) return T2T_ERR_ARG;
+  if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K > (1 << 24) || stuck < MM_STUCK_NONE || stuck > MM_STUCK_RESIDUAL) return T2T_ERR_ARG;
+  if (((uintptr_t)a_codes | (uintptr_t)a_scales | (uintptr_t)w_codes | (uintptr_t)w_scales | (uintptr_t)residual | (uintptr_t)out) % 16)
+    return T2T_ERR_ARG;
+  if (sm_count() < 2) return T2T_ERR_CUDA;
+  const MmPlan plan = mm_plan(M, N, K);
+  if (plan.T && (plan.T != 16 || stuck == MM_STUCK_RESIDUAL)) return T2T_ERR_ARG;
+  MmArgs p = {};
+  p.residual = residual;
+  p.out = out;
+  p.res_row = p.out_row = N;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.wide = true;
+  p.alpha = p.out_scale = p.inv_out_scale = 1.f;
+  p.status = d_status;
+  p.stuck = stuck;
+  MmMaps maps;
+  if (!mm_operand_maps(maps, a_codes, a_scales, w_codes, w_scales, T2T_NVFP4, p, plan)) return T2T_ERR_CUDA;
+  if (plan.T) return mm_launch_rows<T2T_NVFP4, 16, __nv_bfloat16, void, true>(maps, p, plan.splits, stream);
+  if (!mm_result_maps<__nv_bfloat16>(maps, p)) return T2T_ERR_CUDA;
+  return mm_launch_pairs<T2T_NVFP4, __nv_bfloat16, MM_TMA, true>(maps, p, stream);
 }
