@@ -91,3 +91,41 @@ def test_give_up_selftest_refuses_bad_arguments(lib):
     for kw in (dict(stuck=-1), dict(stuck=3), dict(a=0), dict(a=x + 8), dict(M=0), dict(N=0), dict(N=9), dict(K=0), dict(residual=0), dict(out=0),
                dict(out=x + 2), dict(status=0)):
         assert call(**kw) == 1, kw
+
+
+def test_results_that_overlap_a_factor_are_refused(lib):
+    """Other CTAs would still read what the first ones overwrite."""
+    at = dict(a=1 << 20, a_scales=2 << 20, w=3 << 20, w_scales=4 << 20)      # never read
+    M, N, K = 300, 64, 64
+    codes, scales = lib.t2t_fp4_codes_bytes, lib.t2t_fp4_scales_bytes
+
+    def quantised(out, out_scales):
+        return lib.t2t_fp4_matmul_quantize(at["a"], at["a_scales"], at["w"], at["w_scales"], M, N, K, 1, 1.0, 0, 0, 0, 0, 1.0, out,
+                                           out_scales, 0, 0)
+
+    free = 8 << 20
+    for name, size in (("a", codes(M, K)), ("a_scales", scales(M, K, 1)), ("w", codes(N, K)), ("w_scales", scales(N, K, 1))):
+        for p in (at[name], at[name] + size - 16, at[name] - 16):
+            assert quantised(p, free) == 1 and quantised(free, p) == 1, name
+            assert lib.t2t_fp4_matmul(at["a"], at["a_scales"], at["w"], at["w_scales"], M, N, K, 1, 1.0, 0, 0, 0, 0, 0, 0, p, N, 0, 0,
+                                      0) == 1, name
+
+
+def test_residuals_that_the_result_overlaps_are_copied():
+    """But not the result's own, nor other columns of one wide matrix, nor a row for all."""
+    from token2tile_b200.fp4 import _beside
+    wide = torch.arange(20 * 64, dtype=torch.float32).view(20, 64)
+    out = wide[4:12, 16:32]
+    for kept in (out, wide[4:12, :16], wide[4:12, 32:48], wide[:8, 40:56], wide[12:20, 16:32], wide[13:14, :16].expand(8, 16),
+                 torch.zeros(8, 16), wide[11:19, :16], wide[5:13, :16]):
+        assert _beside(kept, out) is kept
+    for other in (wide[5:13, 16:32], wide[3:11, 16:32], wide[4:12, 17:33], wide[4:12, 1:17], wide[11:19, 1:17], wide[0:8, 31:47],
+                  wide[6:7, 20:36].expand(8, 16), wide.view(-1)[4 * 64:][:128].view(8, 16)):
+        got = _beside(other, out)
+        assert got is not other and torch.equal(got, other) and got.untyped_storage().data_ptr() != wide.untyped_storage().data_ptr()
+    one = wide[4:5]      # one row: the stride means nothing
+    assert _beside(wide.view(10, 128)[2:3, :64], one) is not None and _beside(wide[4:5], one) is not None
+    row = wide.view(10, 128)[2:3, :64]
+    assert row.data_ptr() == one.data_ptr() and _beside(row, one) is row
+    half = wide[4:5].clone()
+    assert _beside(half, one) is half and _beside(wide.view(-1)[4 * 64 + 8:][:64].view(1, 64), one).data_ptr() != one.data_ptr() + 32

@@ -622,3 +622,29 @@ def test_status_of_an_earlier_product_is_raised_once():
             call()
         call()
     check_status()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M", [3, 140, 1500])
+def test_results_and_inputs_that_share_memory(fmt, M):
+    """A factor is refused as the result; residuals some of whose elements the result overwrites are read first, by columns and by rows."""
+    N = 1672 if M == 1500 else 264
+    a, w, square = stored(M, 96, fmt, 1), stored(N, 96, fmt, 2), stored(N, N, fmt, 3)
+    b = stored(M, N, fmt, 4)
+    for factors, out in (((b, square), b), ((square, square), square)):
+        with pytest.raises(ValueError, match="shares memory"):
+            fp4_matmul(*factors, out=out)
+    layer = Fp4Linear(w)
+    x = torch.randn(M, 96, generator=gen(5)).to(BF).to(DEV)
+    start = torch.randn(M + 3, N + 24, generator=gen(6)).to(BF).to(DEV)
+    for rows, columns in ((0, 8), (0, 16), (1, 0), (2, 8), (-1, 0), (-3, -8), (0, -8)):
+        r, c = max(-rows, 0), max(-columns, 0)
+        residual = lambda t: t[r:r + M, c:c + N]
+        result = lambda t: t[r + rows:r + rows + M, c + columns:c + columns + N]
+        for call in (lambda **kw: fp4_matmul(a, w, **kw), lambda **kw: layer(x, **kw)):
+            want = call(residual=residual(start).clone())
+            buffer = start.clone()
+            assert torch.equal(call(residual=residual(buffer), out=result(buffer)), want)
+            result(buffer).copy_(result(start))
+            assert torch.equal(buffer, start)
+    check_status()

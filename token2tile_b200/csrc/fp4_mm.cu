@@ -903,6 +903,10 @@ static bool mm_operand_maps(MmMaps& maps, const void* a_codes, const void* a_sca
          make_bytes_tile_map(&maps.w, w_codes, pitch, p.N, 128) &&
          make_scale_map(&maps.sw, w_scales, atoms, cdiv(p.N, 128), box, plan.T ? 1 : 2);
 }
+// Bytes [p, p + n) and [q, q + m) have some in common.
+static bool mm_shares(const void* p, size_t n, const void* q, size_t m) {
+  return (uintptr_t)p < (uintptr_t)q + m && (uintptr_t)q < (uintptr_t)p + n;
+}
 // Checks and launch common to the two entry points; dtype < 0: quantised results.
 static int mm_run(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, int fmt, int dtype,
                   const MmArgs& p, cudaStream_t stream) {
@@ -911,6 +915,15 @@ static int mm_run(const void* a_codes, const void* a_scales, const void* w_codes
   if (!fp4_known(fmt) || !elem_known(p.vec_dtype) || p.act < T2T_ACT_NONE || p.act > T2T_ACT_SILU) return T2T_ERR_ARG;
   if (((uintptr_t)a_codes | (uintptr_t)a_scales | (uintptr_t)w_codes | (uintptr_t)w_scales) % 16) return T2T_ERR_ARG;
   if ((long long)cdiv(p.M, MM_TILE) * cdiv(p.N, MM_TILE) > 0x3fffffffLL) return T2T_ERR_ARG;
+  // factors that the result overlaps would be overwritten while other CTAs still read them
+  const struct { const void* at; size_t bytes; } in[4] = {
+      {a_codes, p.x ? 0 : t2t_fp4_codes_bytes(p.M, p.K)}, {a_scales, p.x ? 0 : t2t_fp4_scales_bytes(p.M, p.K, fmt)},
+      {w_codes, t2t_fp4_codes_bytes(p.N, p.K)}, {w_scales, t2t_fp4_scales_bytes(p.N, p.K, fmt)}};
+  const size_t written = dtype < 0 ? t2t_fp4_codes_bytes(p.M, p.N) : ((p.M - 1) * (size_t)p.out_row + p.N) * elem_bytes(dtype);
+  for (const auto& t : in)
+    if (t.bytes && (mm_shares(t.at, t.bytes, p.out, written) ||
+                    (dtype < 0 && mm_shares(t.at, t.bytes, p.out_scales, t2t_fp4_scales_bytes(p.M, p.N, fmt)))))
+      return T2T_ERR_ARG;
   if (sm_count() < 2) return T2T_ERR_CUDA;
   const MmPlan plan = mm_plan(p.M, p.N, p.K);
   MmMaps maps;

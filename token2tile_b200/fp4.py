@@ -173,6 +173,25 @@ def _vector_type(bias, gate):
     return 0 if vec is None else DTYPES[vec.dtype]
 
 
+def _shares(p, size, q, other):
+    """Two ranges of bytes have some in common."""
+    return p < q + other and q < p + size
+
+
+def _beside(residual, out):
+    """The residual rows, or a copy where some of their elements are other elements of out [M, N]: those would be overwritten before
+    they are read."""
+    (M, N), size, p, q = out.shape, out.element_size(), residual.data_ptr(), out.data_ptr()
+    rs, os = residual.stride(0) if M > 1 else N, out.stride(0) if M > 1 else N
+    if (p == q and rs == os) or not _shares(p, ((M - 1) * rs + N) * size, q, ((M - 1) * os + N) * size):
+        return residual
+    if rs == os:      # columns of one wide matrix: `down` rows and `right` elements further on, or one row more and to the left
+        down, right = divmod(q - p, rs * size)
+        if not (right < N * size and abs(down) < M) and not ((rs * size - right) < N * size and abs(down + 1) < M):
+            return residual
+    return residual.clone()
+
+
 def fp4_quantize(x, fmt="nvfp4", *, tensor_scale=1.0, shift=None, scale=None, eps=1e-6, out=None):
     """x [..., K] as an Fp4Tensor of its rows.  A block's scale comes from its largest magnitude: 2^(floor(log2 top) - 2)
     ("mxfp4") or the 8-bit float next to top / 6 / tensor_scale ("nvfp4"); its elements go to the nearest code, ties to the
@@ -202,7 +221,7 @@ def fp4_quantize(x, fmt="nvfp4", *, tensor_scale=1.0, shift=None, scale=None, ep
 def fp4_matmul(a, w, *, bias=None, activation=None, gate=None, residual=None, dtype=torch.bfloat16, out=None):
     """residual + gate * activation(a w^T + bias) for Fp4Tensors a [M, K] and w [N, K] of one format: [M, N] of `dtype`, summed
     in 32 bits and rounded once.  bias, gate [N] of one type; activation None, "gelu_tanh" or "silu"; residual [M, N] of the
-    result's type; out may be the residual.
+    result's type; out may be the residual, and shares no memory with the other inputs.
 
     dtype "mxfp4" or "nvfp4" (the format of a and w), or an Fp4Tensor [M, N] as out: the result quantised as by fp4_quantize,
     from 32 bits; takes no residual."""
@@ -218,7 +237,10 @@ def fp4_matmul(a, w, *, bias=None, activation=None, gate=None, residual=None, dt
     if codes:
         if residual is not None or (dtype if out is None else out.fmt) != a.fmt:
             raise ValueError(f"a quantised result has the format of its factors, {a.fmt}, and no residual")
-        out = Fp4Tensor.empty(M, N, a.fmt, 1.0, dev) if out is None else out
+        if out is None:
+            out = Fp4Tensor.empty(M, N, a.fmt, 1.0, dev)
+        elif any(_shares(t.data.data_ptr(), t.data.numel(), out.data.data_ptr(), out.data.numel()) for t in (a, w)):
+            raise ValueError("out: shares memory with a factor")
     elif out is None:
         if dtype not in DTYPES:
             raise ValueError(f"dtype: expected bfloat16, float16, float32 or {a.fmt!r}, got {dtype}")
@@ -229,6 +251,8 @@ def fp4_matmul(a, w, *, bias=None, activation=None, gate=None, residual=None, dt
             raise ValueError(f"{name}: expected [{M}, {N}] of the result's type with contiguous rows on {dev}, got {t!r}"[:300])
     if M == 0 or N == 0:
         return out
+    if residual is not None:
+        residual = _beside(residual, out)
     status = _status_of(dev)
     if status.value.value:
         check_status(dev, wait=False)
@@ -323,7 +347,10 @@ def _layer(x, K, last, bias, shift, scale, gate, residual, out, activation, ws_b
         return rows, 0, y, None, None, None
     if _status_of(dev).value.value:
         check_status(dev, wait=False)
-    return (rows, M, y, _rows("out", y), None if residual is None else _rows("residual", residual),
+    to = _rows("out", y)
+    if residual is not None:
+        residual = _rows("residual", residual) if out is None else _beside(_rows("residual", residual), to)
+    return (rows, M, y, to, residual,
             torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None)
 
 
