@@ -648,3 +648,14 @@ def test_results_and_inputs_that_share_memory(fmt, M):
             result(buffer).copy_(result(start))
             assert torch.equal(buffer, start)
     check_status()
+
+
+def test_refused_quantisation_leaves_its_output():
+    x = torch.randn(3, 64, generator=gen(1)).to(DEV)
+    for fmt, bad in (("nvfp4", (0.0, -1.0, math.nan, math.inf, 2.0 ** 101)), ("mxfp4", (2.0, 0.5))):
+        t = fp4_quantize(x, fmt)
+        want = t.dequantize()
+        for g in bad:
+            with pytest.raises(ValueError):
+                fp4_quantize(x, fmt, tensor_scale=g, out=t)
+            assert t.tensor_scale == 1.0 and torch.equal(t.dequantize(), want)

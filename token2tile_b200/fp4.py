@@ -208,10 +208,9 @@ def fp4_quantize(x, fmt="nvfp4", *, tensor_scale=1.0, shift=None, scale=None, ep
         out = Fp4Tensor.empty(M, K, fmt, tensor_scale, x.device)
     elif out.shape != (M, K) or out.fmt != fmt or out.device != x.device:
         raise ValueError(f"out: expected [{M}, {K}] {fmt} on {x.device}, got {out}")
-    else:
-        out.tensor_scale = float(tensor_scale)
     if not 2.0 ** -100 <= tensor_scale <= 2.0 ** 100 or (fmt == "mxfp4" and tensor_scale != 1):
         raise ValueError(f"tensor_scale: expected 1 (mxfp4) or 2^-100 .. 2^100 (nvfp4), got {tensor_scale}")
+    out.tensor_scale = float(tensor_scale)
     if M:
         launch(x.device, "t2t_fp4_quantize", _lib.load().t2t_fp4_quantize, x.data_ptr(), x.stride(0), ptr(shift), ptr(scale), eps, M,
                K, DTYPES[x.dtype], _fmt(fmt), tensor_scale, *out.pointers())
