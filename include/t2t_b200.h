@@ -38,6 +38,7 @@ enum {
 
 /* Element types, 4-bit formats, norms and activations of the operators around the attention. */
 enum { T2T_BF16 = 0, T2T_FP16 = 1, T2T_FP32 = 2 };
+enum { T2T_WIDE_VECTORS = 0x100 };      /* added to dtype, where said: shift and scale have 32 bits */
 enum { T2T_MXFP4 = 0, T2T_NVFP4 = 1 };
 enum { T2T_NORM_NONE = 0, T2T_NORM_HEAD = 1, T2T_NORM_ROW = 2 };
 enum { T2T_ACT_NONE = 0, T2T_ACT_GELU_TANH = 1, T2T_ACT_SILU = 2 };
@@ -338,7 +339,7 @@ size_t t2t_fp4_scales_bytes(int M, int K, int fmt);
 
 /* Quantises x [M, K].  Scale of a block: T2T_MXFP4 2^(floor(log2 top) - 2), T2T_NVFP4 e4m3(top / 6 / tensor_scale), of its
  * largest magnitude top; codes to the nearest, ties to even, saturating at 6.  A block with a NaN or an infinity becomes
- * NaN.  shift, scale [K] (both or none, of x's type): quantises (x - mean) rsqrt(var + eps) (1 + scale) + shift of every
+ * NaN.  shift, scale [K] (both or none, of x's type, of 32 bits with dtype + T2T_WIDE_VECTORS): quantises (x - mean) rsqrt(var + eps) (1 + scale) + shift of every
  * row instead.  tensor_scale: 1 for T2T_MXFP4; 2^-100 .. 2^100, and a power of two if ties are to be exact. */
 int t2t_fp4_quantize(const void* x, long long x_row_stride, const void* shift, const void* scale, float eps, int M, int K,
                      int dtype, int fmt, float tensor_scale, void* codes, void* scales, cudaStream_t stream);
@@ -360,7 +361,7 @@ int t2t_fp4_matmul(const void* a_codes, const void* a_scales, const void* w_code
 int t2t_fp4_matmul_quantize(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, int M,
                             int N, int K, int fmt, float alpha, const void* bias, int act, const void* gate, int vec_dtype,
                             float tensor_scale, void* codes, void* scales, int* d_status, cudaStream_t stream);
-/* A linear layer in one call: x [M, K] quantised as by t2t_fp4_quantize (shift, scale: both or none; tensor scale 1) into the
+/* A linear layer in one call: x [M, K] quantised as by t2t_fp4_quantize (shift, scale, dtype as there; tensor scale 1) into the
  * workspace, then its product with W [N, K] (tensor scale w_scale) as by t2t_fp4_matmul, out and residual of x's type.  ws:
  * t2t_fp4_linear_ws_bytes, 16-byte aligned.  Up to T2T_FP4_FEW_ROWS rows without shift and scale are quantised inside the product, one
  * launch for both, unless out overlaps x; ws may be NULL then. */

@@ -129,3 +129,12 @@ def test_residuals_that_the_result_overlaps_are_copied():
     assert row.data_ptr() == one.data_ptr() and _beside(row, one) is row
     half = wide[4:5].clone()
     assert _beside(half, one) is half and _beside(wide.view(-1)[4 * 64 + 8:][:64].view(1, 64), one).data_ptr() != one.data_ptr() + 32
+
+
+def test_wide_vectors(lib):
+    from token2tile_b200.fp4 import WIDE_VECTORS
+    header = (pathlib.Path(__file__).parents[1] / "include" / "t2t_b200.h").read_text()
+    assert f"T2T_WIDE_VECTORS = {WIDE_VECTORS:#x} " in header
+    x = 4096                     # never read
+    for dtype in (3, WIDE_VECTORS + 3, WIDE_VECTORS * 2, -1):
+        assert lib.t2t_fp4_quantize(x, 64, x, x, 1e-6, 4, 64, dtype, 1, 1.0, x, x, 0) == 1

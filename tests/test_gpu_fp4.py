@@ -659,3 +659,39 @@ def test_refused_quantisation_leaves_its_output():
             with pytest.raises(ValueError):
                 fp4_quantize(x, fmt, tensor_scale=g, out=t)
             assert t.tensor_scale == 1.0 and torch.equal(t.dequantize(), want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M,K", [(1, 16), (3, 48), (130, 256), (9, 1000), (33, 5120), (700, 1001), (5, 16384), (5, 20481), (2, 30001)])
+def test_modulated_quantize_with_wide_vectors(fmt, dtype, M, K):
+    """32-bit shift and scale with rows of any type: values of x's type give the bits that they give as x's type; others what
+    the formula gives, as near as in test_modulated_quantize."""
+    g = gen(M + K)
+    x = (torch.randn(M, K, generator=g) * 3 + torch.randn(M, 1, generator=g)).to(dtype)
+    shift, scale = ((0.2 * torch.randn(K, generator=g)).to(dtype).to(DEV) for _ in range(2))
+    codes = lambda **kw: fp4_quantize(x.to(DEV), fmt, **kw).to_stored()
+    for a, b in zip(codes(shift=shift, scale=scale), codes(shift=shift.float(), scale=scale.float())):
+        assert torch.equal(a, b)
+    weight = torch.rand(K, generator=g) * 0.015 + 0.005      # of a norm: 16 bits do not hold its distance from 1
+    shift = 0.01 * torch.randn(K, generator=g)
+    t = fp4_quantize(x.to(DEV), fmt, shift=shift.to(DEV), scale=(weight - 1).to(DEV))
+    y = plain64.modulated(x.double(), shift.double(), weight.double() - 1)
+    _, s, value = plain64.quantize(y, fmt)
+    got = values(t)
+    # these rows lie where nvfp4's scales are subnormal and the definition itself is off by more than a step
+    step = (s.repeat_interleave(plain64.BLOCK[fmt], 1)[:, :K]) * 2 * 1.2
+    assert bool(((got - y).abs() <= (value - y).abs() + step * (2 if fmt == "mxfp4" else 1) + 1e-30).all())
+    # weight - 1 in 32 bits is off by 2^-25, 6e-6 of the weight at most: one value in some thousand next to a middle or a scale's
+    assert float((got != value).double().mean()) < 5e-3 + 40.0 / (M * K) * (M * K < 40000)
+    layer = Fp4Linear((torch.randn(40, K, generator=g) / K ** 0.5).to(DEV), fmt=fmt)
+    both = dict(shift=shift.to(DEV), scale=(weight - 1).to(DEV))
+    assert torch.equal(layer(x.to(DEV), **both), layer(t, dtype=dtype))
+    back = Fp4Linear(torch.randn(8, 40, generator=g).to(DEV), fmt=fmt)
+    assert torch.equal(Fp4FeedForward(layer, back)(x.to(DEV), **both),
+                       fp4_matmul(fp4_matmul(t, layer.w, activation="gelu_tanh", dtype=fmt), back.w, dtype=dtype))
+    for bad in (dict(shift=shift.to(DEV).to(F16), scale=(weight - 1).to(DEV)), dict(shift=shift.to(DEV).double(), scale=shift.to(DEV).double())):
+        for call in (lambda: fp4_quantize(x.to(DEV), fmt, **bad), lambda: layer(x.to(DEV), **bad)):
+            with pytest.raises(ValueError):
+                call()
+    check_status()

@@ -61,6 +61,13 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* __restrict__
   }
 }
 
+// 16 elements of a shift or scale from column `at`: of x's type, or of 32 bits.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_vector(const void* v, bool wide, int at, int K, float* y) {
+  if (sizeof(T) == 2 && wide) load16<float, VEC>(static_cast<const float*>(v) + at, K - at, y);
+  else load16<T, VEC>(static_cast<const T*>(v) + at, K - at, y);
+}
+
 // Modulated rows.  A thread owns U x 16 columns and walks down the CTA's rows, R at a time, the next ones on their way meanwhile; shift
 // and 1 + scale lie in shared memory in 32 bits, read once for all R.  Mean, then mean square about it, from registers: one pass over x.
 // Bound by instructions and the latency of its sums (two meetings of the block for R rows): 75,600 x 5,120 bf16 nvfp4 takes 255 us,
@@ -95,8 +102,8 @@ __device__ __forceinline__ void mod_sums(float (&v)[R], float (&to)[R][32]) {
 }
 template <typename T, int FMT, bool VEC, int U, int R>
 __global__ void __launch_bounds__(mod_threads(U, R), U == 1 ? 2 : 1)
-    fp4_modulate_kernel(const T* __restrict__ x, long long x_row, int M, int K, const T* __restrict__ shift,
-                        const T* __restrict__ scale, float eps, float g, float inv_g, int rows, int pitch, int atoms,
+    fp4_modulate_kernel(const T* __restrict__ x, long long x_row, int M, int K, const void* __restrict__ shift,
+                        const void* __restrict__ scale, bool wide, float eps, float g, float inv_g, int rows, int pitch, int atoms,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr int B = fp4_block(FMT);
   static_assert(R == 1 || mod_threads(U, R) <= 512, "mod_sums: a half warp takes the warps' sums");
@@ -110,8 +117,8 @@ __global__ void __launch_bounds__(mod_threads(U, R), U == 1 ? 2 : 1)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float m[16], s[16];
-    load16<T, VEC>(scale + column(u), K - column(u), m);
-    load16<T, VEC>(shift + column(u), K - column(u), s);
+    load_vector<T, VEC>(scale, wide, column(u), K, m);
+    load_vector<T, VEC>(shift, wide, column(u), K, s);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       vector(0, u, c) = make_ulonglong2(pair_of(1.f + m[4 * c], 1.f + m[4 * c + 1]), pair_of(1.f + m[4 * c + 2], 1.f + m[4 * c + 3]));
@@ -197,10 +204,10 @@ __global__ void __launch_bounds__(mod_threads(U, R), U == 1 ? 2 : 1)
   }
 }
 
-// The same for rows that are too long for a block's registers: 256 threads a row, every look reads it again.
-template <typename T, int FMT, bool VEC>
+// The same for rows that are too long for a block's registers: 256 threads a row, every look reads it again.  WIDE: 32-bit vectors.
+template <typename T, int FMT, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(256) fp4_modulate_long_kernel(const T* __restrict__ x, long long x_row, int K,
-                                                                const T* __restrict__ shift, const T* __restrict__ scale,
+                                                                const void* __restrict__ shift, const void* __restrict__ scale,
                                                                 float eps, float g, float inv_g, int pitch, int atoms,
                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   __shared__ float red[2][8];
@@ -235,8 +242,8 @@ __global__ void __launch_bounds__(256) fp4_modulate_long_kernel(const T* __restr
     const int at = u + threadIdx.x * 16;
     float y[16], sc[16], sh[16];
     load16<T, VEC>(p + at, K - at, y);
-    load16<T, VEC>(scale + at, K - at, sc);
-    load16<T, VEC>(shift + at, K - at, sh);
+    load_vector<T, VEC>(scale, WIDE, at, K, sc);
+    load_vector<T, VEC>(shift, WIDE, at, K, sh);
 #pragma unroll
     for (int e = 0; e < 16; ++e) y[e] = at + e < K ? fmaf((y[e] - mean) * r, 1.f + sc[e], sh[e]) : 0.f;
     put_unit<FMT, false>(y, at < width, row, at, pitch, atoms, g, inv_g, codes, scales);
@@ -319,8 +326,8 @@ static int rows_per_cta(int M, int blocks) {
 static int mod_block(int K, int fmt, int U) { return cdiv(4 * fp4_atoms(K, fmt) * fp4_block(fmt) / 16, 32 * U) * 32; }
 
 template <typename T, int FMT, bool VEC, int U, int R>
-static int modulate_t(const T* x, long long x_row, int M, int K, const T* shift, const T* scale, float eps, float g, uint8_t* codes,
-                      uint8_t* scales, cudaStream_t st) {
+static int modulate_t(const T* x, long long x_row, int M, int K, const void* shift, const void* scale, bool wide, float eps, float g,
+                      uint8_t* codes, uint8_t* scales, cudaStream_t st) {
   const int threads = mod_block(K, FMT, U), smem = 2 * U * 4 * threads * 16;
   auto* k = fp4_modulate_kernel<T, FMT, VEC, U, R>;
   static std::atomic<unsigned long long> allowed{0};
@@ -329,16 +336,16 @@ static int modulate_t(const T* x, long long x_row, int M, int K, const T* shift,
   const int by_regs = 65536 / (mod_regs(U, R) * threads), by_smem = 224 * 1024 / (smem + 2048), by_slots = 32;
   const int ctas = by_regs < by_smem ? (by_regs < by_slots ? by_regs : by_slots) : (by_smem < by_slots ? by_smem : by_slots);
   const int share = cdiv(M, 148 * (ctas > 1 ? ctas : 1)), rows = share > R ? share : R;
-  k<<<cdiv(M, rows), threads, smem, st>>>(x, x_row, M, K, shift, scale, eps, g, 1.f / g, rows, fp4_pitch(K), fp4_atoms(K, FMT), codes,
-                                          scales);
+  k<<<cdiv(M, rows), threads, smem, st>>>(x, x_row, M, K, shift, scale, wide, eps, g, 1.f / g, rows, fp4_pitch(K), fp4_atoms(K, FMT),
+                                          codes, scales);
   return cudaGetLastError() == cudaSuccess ? T2T_OK : T2T_ERR_CUDA;
 }
 
 template <typename T, int FMT>
-static int quantize_t(const void* x, long long x_row, int M, int K, const void* shift, const void* scale, float eps, float g,
-                      uint8_t* codes, uint8_t* scales, cudaStream_t st) {
+static int quantize_t(const void* x, long long x_row, int M, int K, const void* shift, const void* scale, bool wide, float eps,
+                      float g, uint8_t* codes, uint8_t* scales, cudaStream_t st) {
   const int pitch = fp4_pitch(K), atoms = fp4_atoms(K, FMT);
-  const T *p = static_cast<const T*>(x), *sh = static_cast<const T*>(shift), *sc = static_cast<const T*>(scale);
+  const T* p = static_cast<const T*>(x);
   const uintptr_t at = (uintptr_t)x | (uintptr_t)shift | (uintptr_t)scale;
   const bool vec = at % 16 == 0 && x_row * (long long)sizeof(T) % 16 == 0;
   if (shift) {
@@ -348,16 +355,18 @@ static int quantize_t(const void* x, long long x_row, int M, int K, const void* 
     // (32,759 x 5,119 fp16: 226 and 205).
     if constexpr (sizeof(T) == 2) {
       if (vec && mod_block(K, FMT, 1) <= mod_threads(1, 2))
-        return modulate_t<T, FMT, true, 1, 2>(p, x_row, M, K, sh, sc, eps, g, codes, scales, st);
+        return modulate_t<T, FMT, true, 1, 2>(p, x_row, M, K, shift, scale, wide, eps, g, codes, scales, st);
       if (vec && mod_block(K, FMT, 2) <= mod_threads(2, 2))
-        return modulate_t<T, FMT, true, 2, 2>(p, x_row, M, K, sh, sc, eps, g, codes, scales, st);
+        return modulate_t<T, FMT, true, 2, 2>(p, x_row, M, K, shift, scale, wide, eps, g, codes, scales, st);
     }
     if (mod_block(K, FMT, 2) <= mod_threads(2, 1)) {
-      if (vec) return modulate_t<T, FMT, true, 2, 1>(p, x_row, M, K, sh, sc, eps, g, codes, scales, st);
-      return modulate_t<T, FMT, false, 2, 1>(p, x_row, M, K, sh, sc, eps, g, codes, scales, st);
+      if (vec) return modulate_t<T, FMT, true, 2, 1>(p, x_row, M, K, shift, scale, wide, eps, g, codes, scales, st);
+      return modulate_t<T, FMT, false, 2, 1>(p, x_row, M, K, shift, scale, wide, eps, g, codes, scales, st);
     }
-    auto* k = vec ? fp4_modulate_long_kernel<T, FMT, true> : fp4_modulate_long_kernel<T, FMT, false>;
-    k<<<M, 256, 0, st>>>(p, x_row, K, sh, sc, eps, g, 1.f / g, pitch, atoms, codes, scales);
+    constexpr bool narrow = sizeof(T) == 2;
+    auto* k = wide && narrow ? (vec ? fp4_modulate_long_kernel<T, FMT, true, narrow> : fp4_modulate_long_kernel<T, FMT, false, narrow>)
+                             : (vec ? fp4_modulate_long_kernel<T, FMT, true, false> : fp4_modulate_long_kernel<T, FMT, false, false>);
+    k<<<M, 256, 0, st>>>(p, x_row, K, shift, scale, eps, g, 1.f / g, pitch, atoms, codes, scales);
   } else {
     const int rows = rows_per_cta(M, atoms * (fp4_block(FMT) / 4));
     auto* k = vec ? fp4_quantize_kernel<T, FMT, true> : fp4_quantize_kernel<T, FMT, false>;
@@ -392,14 +401,16 @@ extern "C" size_t t2t_fp4_scales_bytes(int M, int K, int fmt) {
 
 extern "C" int t2t_fp4_quantize(const void* x, long long x_row_stride, const void* shift, const void* scale, float eps, int M,
                                 int K, int dtype, int fmt, float tensor_scale, void* codes, void* scales, cudaStream_t stream) {
+  const bool wide = dtype & T2T_WIDE_VECTORS;
+  dtype &= ~T2T_WIDE_VECTORS;
   if (!x || !codes || !scales || !fp4_shape_ok(M, K) || !elem_known(dtype) || !fp4_known(fmt)) return T2T_ERR_ARG;
   if (!shift != !scale || x_row_stride < 0 || (uintptr_t)codes % 16) return T2T_ERR_ARG;
   if (!(tensor_scale >= 0x1p-100f && tensor_scale <= 0x1p100f) || (fmt == T2T_MXFP4 && tensor_scale != 1.f)) return T2T_ERR_ARG;
   uint8_t *c = static_cast<uint8_t*>(codes), *s = static_cast<uint8_t*>(scales);
 #define T2T_CALL(T)                                                                                                       \
   return fmt == T2T_MXFP4                                                                                                 \
-             ? quantize_t<T, T2T_MXFP4>(x, x_row_stride, M, K, shift, scale, eps, tensor_scale, c, s, stream)             \
-             : quantize_t<T, T2T_NVFP4>(x, x_row_stride, M, K, shift, scale, eps, tensor_scale, c, s, stream)
+             ? quantize_t<T, T2T_MXFP4>(x, x_row_stride, M, K, shift, scale, wide, eps, tensor_scale, c, s, stream)             \
+             : quantize_t<T, T2T_NVFP4>(x, x_row_stride, M, K, shift, scale, wide, eps, tensor_scale, c, s, stream)
   if (dtype == T2T_BF16) T2T_CALL(__nv_bfloat16);
   if (dtype == T2T_FP16) T2T_CALL(__half);
   T2T_CALL(float);

@@ -984,6 +984,8 @@ extern "C" int t2t_fp4_matmul_quantize(const void* a_codes, const void* a_scales
 // in x's type, or null; where it overlaps x, some CTAs would write what others have yet to read.
 static int mm_input(MmInput& a, const void* x, long long x_row, const void* shift, const void* scale, float eps, int M, int K, int dtype,
                     int fmt, const void* out, long long out_row, int N, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  const int vectors = dtype & T2T_WIDE_VECTORS;
+  dtype &= ~T2T_WIDE_VECTORS;
   if (!x || x_row < 0 || !elem_known(dtype)) return T2T_ERR_ARG;
   auto end = [&](const void* y, long long row, int n) { return (uintptr_t)y + ((M - 1) * row + n) * elem_bytes(dtype); };
   const bool apart = !out || end(x, x_row, K) <= (uintptr_t)out || end(out, out_row, N) <= (uintptr_t)x;
@@ -993,7 +995,7 @@ static int mm_input(MmInput& a, const void* x, long long x_row, const void* shif
   if (ws_bytes < t2t_fp4_linear_ws_bytes(M, K, fmt)) return T2T_ERR_WORKSPACE;
   uint8_t* scales = static_cast<uint8_t*>(ws) + t2t_fp4_codes_bytes(M, K);
   a = {ws, scales, nullptr, 0, 0};
-  return t2t_fp4_quantize(x, x_row, shift, scale, eps, M, K, dtype, fmt, 1.f, ws, scales, stream);
+  return t2t_fp4_quantize(x, x_row, shift, scale, eps, M, K, dtype | vectors, fmt, 1.f, ws, scales, stream);
 }
 
 extern "C" size_t t2t_fp4_linear_ws_bytes(int M, int K, int fmt) {
@@ -1010,7 +1012,7 @@ extern "C" int t2t_fp4_linear(const void* x, long long x_row_stride, const void*
   const int rc = mm_input(a, x, x_row_stride, shift, scale, eps, M, K, dtype, fmt, out, out_row_stride, N, ws, ws_bytes, stream);
   if (rc != T2T_OK) return rc;
   return mm_values(a, w_codes, w_scales, M, N, K, fmt, w_scale, bias, act, gate, vec_dtype, residual, residual_row_stride, out,
-                   out_row_stride, dtype, d_status, stream);
+                   out_row_stride, dtype & ~T2T_WIDE_VECTORS, d_status, stream);
 }
 
 extern "C" size_t t2t_fp4_feed_forward_ws_bytes(int M, int K, int F, int fmt) {
@@ -1032,7 +1034,7 @@ extern "C" int t2t_fp4_feed_forward(const void* x, long long x_row_stride, const
   rc = mm_codes(a, up_codes, up_scales, M, F, K, fmt, up_scale, up_bias, act, nullptr, up_vec_dtype, 1.f, h, hs, d_status, stream);
   if (rc != T2T_OK) return rc;
   return t2t_fp4_matmul(h, hs, down_codes, down_scales, M, N, F, fmt, down_scale, down_bias, T2T_ACT_NONE, gate, down_vec_dtype,
-                        residual, residual_row_stride, out, out_row_stride, dtype, d_status, stream);
+                        residual, residual_row_stride, out, out_row_stride, dtype & ~T2T_WIDE_VECTORS, d_status, stream);
 }
 
 extern "C" int t2t_fp4_give_up_selftest(int stuck, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,

@@ -150,7 +150,7 @@ class DiTBlock:
         q, k = self._norm_and_turn(self.q(h, dtype=x.dtype), self.k(h, dtype=x.dtype), positions, rotary)
         v = self.v(h, dtype=x.dtype).view(-1, self.shape.heads, self.shape.head_dim)
         x = self.o(self._attend(q, k, v, attn_metadata, group), gate=gate_sa, residual=x)
-        cq = self.cq(x, shift=self.norm3_b, scale=self.norm3_w - 1)
+        cq = self.cq(x, shift=self.norm3_b.float(), scale=self.norm3_w.float() - 1)
         x = self.co(self._cross(cq, self.ck(text, dtype=x.dtype), self.cv(text, dtype=x.dtype)), residual=x)
         return self.ffn(x, shift=shift_ff, scale=scale_ff, gate=gate_ff, residual=x)
 

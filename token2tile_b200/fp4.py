@@ -23,6 +23,7 @@ FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 ACTIVATIONS = {None: 0, "gelu_tanh": 1, "silu": 2}
 FEW_ROWS = 4      # T2T_FP4_FEW_ROWS
+WIDE_VECTORS = 0x100      # T2T_WIDE_VECTORS
 
 
 class _Status:
@@ -168,6 +169,18 @@ def _vector(name, v, n, dev, dtype=None):
                          f"on {v.device}")
 
 
+def _modulation(shift, scale, K, dev, dtype):
+    """Checks of shift and scale; the C entries' type of an x of `dtype` with them."""
+    if shift is None and scale is None:
+        return DTYPES[dtype]
+    if shift is None or scale is None:
+        raise ValueError("shift and scale are given together")
+    kind = torch.float32 if shift.dtype == torch.float32 else dtype
+    _vector("shift", shift, K, dev, kind)
+    _vector("scale", scale, K, dev, kind)
+    return DTYPES[dtype] if kind == dtype else DTYPES[dtype] | WIDE_VECTORS
+
+
 def _vector_type(bias, gate):
     vec = bias if bias is not None else gate
     return 0 if vec is None else DTYPES[vec.dtype]
@@ -197,13 +210,11 @@ def fp4_quantize(x, fmt="nvfp4", *, tensor_scale=1.0, shift=None, scale=None, ep
     ("mxfp4") or the 8-bit float next to top / 6 / tensor_scale ("nvfp4"); its elements go to the nearest code, ties to the
     even one, saturating at 6.  A block with a NaN or an infinity is NaN as a whole.
 
-    shift, scale [K]: quantises layer_norm(x) * (1 + scale) + shift, which is never written out."""
+    shift, scale [K] of x's type or float32: quantises layer_norm(x) * (1 + scale) + shift, which is never written out.  (A norm's
+    weight w as scale = w - 1 is given in float32: in 16 bits the difference loses what w has below 2^-8.)"""
     x = _rows("x", x)
     M, K = x.shape
-    if (shift is None) != (scale is None):
-        raise ValueError("shift and scale are given together")
-    _vector("shift", shift, K, x.device, x.dtype)
-    _vector("scale", scale, K, x.device, x.dtype)
+    kind = _modulation(shift, scale, K, x.device, x.dtype)
     if out is None:
         out = Fp4Tensor.empty(M, K, fmt, tensor_scale, x.device)
     elif out.shape != (M, K) or out.fmt != fmt or out.device != x.device:
@@ -213,7 +224,7 @@ def fp4_quantize(x, fmt="nvfp4", *, tensor_scale=1.0, shift=None, scale=None, ep
     out.tensor_scale = float(tensor_scale)
     if M:
         launch(x.device, "t2t_fp4_quantize", _lib.load().t2t_fp4_quantize, x.data_ptr(), x.stride(0), ptr(shift), ptr(scale), eps, M,
-               K, DTYPES[x.dtype], _fmt(fmt), tensor_scale, *out.pointers())
+               K, kind, _fmt(fmt), tensor_scale, *out.pointers())
     return out
 
 
@@ -289,7 +300,7 @@ class Fp4Linear:
         self.b = bias
 
     def __call__(self, x, *, shift=None, scale=None, eps=1e-6, activation=None, gate=None, residual=None, out=None, dtype=None):
-        """x [..., in] -> [..., out] of x's type.  shift, scale [in]: of layer_norm(x) * (1 + scale) + shift.
+        """x [..., in] -> [..., out] of x's type.  shift, scale [in] of that type or float32: of layer_norm(x) * (1 + scale) + shift.
         gate [out], residual and out [..., out]: residual + gate * (...).  x may be an Fp4Tensor [rows, in] that several layers
         share (fp4_quantize); the result is then of `dtype` (bfloat16)."""
         if isinstance(x, Fp4Tensor):
@@ -304,12 +315,12 @@ class Fp4Linear:
             raise ValueError(f"x: expected [..., {K}], got {tuple(x.shape)}")
         w = self.w
         inside = out is None and shift is None and math.prod(x.shape[:-1]) <= FEW_ROWS      # quantised by the product
-        rows, M, y, to, res, ws = _layer(x, K, w, self.b, shift, scale, gate, residual, out, activation,
-                                         0 if inside else _bytes(x.shape, K, w.fmt))
+        rows, kind, M, y, to, res, ws = _layer(x, K, w, self.b, shift, scale, gate, residual, out, activation,
+                                               0 if inside else _bytes(x.shape, K, w.fmt))
         if M:
             dev = w.device
             launch(dev, "t2t_fp4_linear", _lib.load().t2t_fp4_linear, rows.data_ptr(), rows.stride(0), ptr(shift), ptr(scale), eps, M,
-                   K, DTYPES[x.dtype], FORMATS[w.fmt], *w.pointers(), w.tensor_scale, w.shape[0], ptr(self.b),
+                   K, kind, FORMATS[w.fmt], *w.pointers(), w.tensor_scale, w.shape[0], ptr(self.b),
                    ACTIVATIONS[activation], ptr(gate), _vector_type(self.b, gate), ptr(res), 0 if res is None else res.stride(0),
                    to.data_ptr(), to.stride(0) if M > 1 else w.shape[0], ptr(ws), 0 if ws is None else ws.shape[0], _status_of(dev).ptr)
         return y
@@ -322,8 +333,8 @@ def _bytes(shape, K, fmt):
 
 
 def _layer(x, K, last, bias, shift, scale, gate, residual, out, activation, ws_bytes):
-    """Checks of a layer whose last product is with `last`, and what it needs: x and out as rows, their number (0: nothing to do),
-    the result, residual rows, workspace."""
+    """Checks of a layer whose last product is with `last`, and what it needs: x as rows, its type with the vectors', the rows' number (0:
+    nothing to do), the result, it and the residual as rows, workspace."""
     dev, shape = last.device, (*x.shape[:-1], last.shape[0])
     N = shape[-1]
     if x.device != dev:
@@ -331,11 +342,7 @@ def _layer(x, K, last, bias, shift, scale, gate, residual, out, activation, ws_b
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     rows = _rows("x", x)
-    if shift is not None or scale is not None:
-        if shift is None or scale is None:
-            raise ValueError("shift and scale are given together")
-        _vector("shift", shift, K, dev, x.dtype)
-        _vector("scale", scale, K, dev, x.dtype)
+    kind = _modulation(shift, scale, K, dev, x.dtype)
     _vector("gate", gate, N, dev, None if bias is None else bias.dtype)
     for name, t in (("residual", residual), ("out", out)):
         if t is not None and (t.shape != shape or t.dtype != x.dtype or t.device != dev):
@@ -343,13 +350,13 @@ def _layer(x, K, last, bias, shift, scale, gate, residual, out, activation, ws_b
     y = torch.empty(*shape, dtype=x.dtype, device=dev) if out is None else out
     M = rows.shape[0]
     if M == 0 or N == 0:
-        return rows, 0, y, None, None, None
+        return rows, kind, 0, y, None, None, None
     if _status_of(dev).value.value:
         check_status(dev, wait=False)
     to = _rows("out", y)
     if residual is not None:
         residual = _rows("residual", residual) if out is None else _beside(_rows("residual", residual), to)
-    return (rows, M, y, to, residual,
+    return (rows, kind, M, y, to, residual,
             torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None)
 
 
@@ -371,12 +378,12 @@ class Fp4FeedForward:
         up, down = self.up, self.down
         u, d = up.w, down.w
         F, N = d.shape[1], d.shape[0]
-        rows, M, y, to, res, ws = _layer(x, K, d, down.b, shift, scale, gate, residual, out, self.activation,
-                                         _bytes(x.shape, K, u.fmt) + _bytes(x.shape, F, u.fmt))
+        rows, kind, M, y, to, res, ws = _layer(x, K, d, down.b, shift, scale, gate, residual, out, self.activation,
+                                               _bytes(x.shape, K, u.fmt) + _bytes(x.shape, F, u.fmt))
         if M:
             dev = u.device
             launch(dev, "t2t_fp4_feed_forward", _lib.load().t2t_fp4_feed_forward, rows.data_ptr(), rows.stride(0), ptr(shift),
-                   ptr(scale), eps, M, K, DTYPES[x.dtype], FORMATS[u.fmt], *u.pointers(), u.tensor_scale, F, ptr(up.b),
+                   ptr(scale), eps, M, K, kind, FORMATS[u.fmt], *u.pointers(), u.tensor_scale, F, ptr(up.b),
                    _vector_type(up.b, None), ACTIVATIONS[self.activation], *d.pointers(), d.tensor_scale, N, ptr(down.b), ptr(gate),
                    _vector_type(down.b, gate), ptr(res), 0 if res is None else res.stride(0), to.data_ptr(),
                    to.stride(0) if M > 1 else N, ws.data_ptr(), ws.shape[0], _status_of(dev).ptr)
