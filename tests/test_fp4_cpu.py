@@ -138,3 +138,31 @@ def test_wide_vectors(lib):
     x = 4096                     # never read
     for dtype in (3, WIDE_VECTORS + 3, WIDE_VECTORS * 2, -1):
         assert lib.t2t_fp4_quantize(x, 64, x, x, 1e-6, 4, 64, dtype, 1, 1.0, x, x, 0) == 1
+
+
+def test_a_device_has_one_status_word(monkeypatch):
+    """Threads whose first calls meet get the same word: kernels of both write to what either reads."""
+    import threading
+    import time
+    import types
+
+    from token2tile_b200 import fp4
+
+    class Slow:
+        def __init__(self):
+            time.sleep(0.05)
+
+    monkeypatch.setattr(fp4, "_Status", Slow)
+    monkeypatch.setattr(fp4, "_status", {})
+    start, got = threading.Barrier(8), []
+
+    def ask(index):
+        start.wait()
+        got.append((index, fp4._status_of(types.SimpleNamespace(index=index))))
+
+    threads = [threading.Thread(target=ask, args=(i % 2,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 8 and all(s is fp4._status[i] for i, s in got) and fp4._status[0] is not fp4._status[1]

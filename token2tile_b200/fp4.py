@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -36,12 +37,16 @@ class _Status:
 
 
 _status: dict = {}
+_status_lock = threading.Lock()      # queued kernels point to the word: a device has one, whichever thread asks first
 
 
 def _status_of(dev):
     s = _status.get(dev.index)
     if s is None:
-        s = _status[dev.index] = _Status()
+        with _status_lock:
+            s = _status.get(dev.index)
+            if s is None:
+                s = _status[dev.index] = _Status()
     return s
 
 
