@@ -267,3 +267,67 @@ def test_rotated_part_of_whole_vectors(case):
     """The rotated part ends at a vector, but not at a pair of them."""
     test_forward_and_gradient(case, 0)
     test_forward_and_gradient(case, 2)
+
+
+@pytest.mark.parametrize("norm", ["", "head", "row"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("keys", [0, 3])
+def test_autograd(norm, dtype, keys):
+    """Gradients through torch.autograd are those of backward, with gradients of any strides; nothing is cut off silently."""
+    gen = torch.Generator().manual_seed(12)
+    rot = Rotary(64, 32, layout="half")
+    pos = torch.arange(9, device=DEV) + 100
+    q, k = make((9, 6, 64), dtype, gen, True, 3)
+    k = k if keys else None
+    dq, dk = make((9, 6, 64), dtype, gen, False, 3)
+    w = [None, None]
+    if norm:
+        w = [(1 + 0.2 * torch.randn(n, generator=gen)).to(dtype).to(DEV) for n in ((64, 64) if norm == "head" else (6 * 64, 3 * 64))]
+    if not keys:
+        w[1] = None
+    want = rot.backward(dq, dk if keys else None, pos, q=q, k=k, q_weight=w[0], k_weight=w[1])
+    leaf = [None if t is None else t.detach().clone().requires_grad_() for t in (q, k, *w)]
+    outs = rot(leaf[0], leaf[1], pos, q_weight=leaf[2], k_weight=leaf[3])
+    assert torch.equal(outs[0], rot(q, k, pos, q_weight=w[0], k_weight=w[1])[0])
+    torch.autograd.backward([t for t in outs if t is not None], [dq, dk][:1 + bool(keys)])
+    for x, g in zip(leaf, want):
+        assert (x is None) == (g is None) and (x is None or torch.equal(x.grad, g.to(x.dtype)))
+    # an expanded gradient, one output alone, and one input or weight alone
+    x = q.detach().clone().requires_grad_()
+    rot(x, k, pos, q_weight=w[0], k_weight=w[1])[0].sum().backward()
+    ones = rot.backward(torch.ones_like(q), None if k is None else torch.zeros_like(k), pos, q=q, k=k, q_weight=w[0], k_weight=w[1])
+    assert torch.equal(x.grad, ones[0])
+    if norm:
+        x = w[0].detach().clone().requires_grad_()
+        rot(q, k, pos, q_weight=x, k_weight=w[1])[0].backward(dq)
+        assert torch.equal(x.grad, rot.backward(dq, None if k is None else torch.zeros_like(k), pos, q=q, k=k, q_weight=w[0],
+                                                k_weight=w[1])[2].to(dtype))
+    else:
+        x = q.detach().clone().requires_grad_()
+        rot(x, k, pos, inverse=True)[0].backward(dq)
+        assert torch.equal(x.grad, rot(dq, None, pos)[0])
+    with torch.no_grad():
+        assert not rot(leaf[0], None, pos)[0].requires_grad
+
+
+def test_writing_to_out_is_seen_by_autograd():
+    rot = Rotary(64)
+    pos = torch.arange(5, device=DEV)
+    q, k = make((5, 4, 64), F32, torch.Generator().manual_seed(13), False, 4)
+    w = torch.rand(64, device=DEV, requires_grad=True)
+    loss = (q * w).sum()      # saves q
+    rot(q, k, pos, out=(q, k))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    dq, dk, one = torch.ones_like(q), torch.ones_like(k), torch.ones(64, device=DEV)
+    loss = (dq * w).sum()
+    rot.backward(dq, dk, pos, q=q, k=k, q_weight=one, k_weight=one, out=(dq, dk))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    for kw in (dict(out=(torch.empty_like(q), torch.empty_like(k)), q_weight=w, k_weight=w),
+               dict(out=(torch.empty_like(q).requires_grad_(), torch.empty_like(k)))):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            rot(q, k, pos, **kw)
+    with torch.inference_mode():
+        x, y = q.clone(), k.clone()
+        assert rot(x, y, pos, out=(x, y))[0] is x

@@ -4,7 +4,7 @@
     q, k = rot(q, k, positions, q_weight=wq, k_weight=wk)            # q, k [N, H, 128]; positions [3, N]
 
 One kernel turns q and k together (t2t_rotary): every head's pairs by the angle position * frequency, in 32 bits, rounded
-once.  The reference leaves positions to its host.
+once.  Gradients of q, k and the weights pass through it (torch.autograd).  The reference leaves positions to its host.
 """
 from __future__ import annotations
 
@@ -12,6 +12,8 @@ import math
 import struct
 
 import torch
+
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._launch import DTYPES, launch
@@ -76,6 +78,28 @@ def _layout(name, t):
     if st[-1] != 1 and t.shape[-1] != 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous, got strides {tuple(st)}")
     return (0, st[0], st[1]) if len(st) == 3 else st[:3]
+
+
+class _Turned(torch.autograd.Function):
+    """Rotary.__call__ where autograd wants gradients of its inputs."""
+
+    @staticmethod
+    def forward(ctx, rot, q, k, positions, q_weight, k_weight, eps, inverse):
+        ctx.rot, ctx.eps, ctx.inverse = rot, eps, inverse
+        normed = q_weight is not None
+        ctx.save_for_backward(q if normed else None, k if normed else None, positions, q_weight, k_weight)
+        return rot(q, k, positions, q_weight=q_weight, k_weight=k_weight, eps=eps, inverse=inverse)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, positions, q_weight, k_weight = ctx.saved_tensors
+        # autograd hands over expanded gradients too
+        dq, dk = (d if d is None or d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
+        if q_weight is None:
+            return (None, *ctx.rot(dq, dk, positions, inverse=not ctx.inverse), *[None] * 5)
+        dq, dk, dwq, dwk = ctx.rot.backward(dq, dk, positions, q=q, k=k, q_weight=q_weight, k_weight=k_weight, eps=ctx.eps)
+        return None, dq, dk, None, dwq.to(q_weight.dtype), None if k_weight is None else dwk.to(k_weight.dtype), None, None
 
 
 _STRIDES4, _STRIDES6 = struct.Struct("12q"), struct.Struct("18q")      # as the C entries take them
@@ -191,12 +215,22 @@ class Rotary:
         """q [N, H, D] or [B, N, H, D] and k (the same with its own number of heads, or None), positions int32 or int64
         [N] or [B, N], with axes [A, N] or [A, B, N].  Any strides with contiguous heads.  q_weight, k_weight [D] or
         [H * D]: RMS norm over each head or over all heads of a token in front of the rotation.  inverse: turns back,
-        which without a norm is the gradient.  out: (q, k) to write to, which may be the inputs.  Returns (q, k)."""
-        positions, B, N, pa, pb = self._common(q, k, positions)
+        which without a norm is the gradient.  out: (q, k) to write to, which may be the inputs and share no other memory with
+        them; not where autograd wants a gradient.  Returns (q, k)."""
+        checked, B, N, pa, pb = self._common(q, k, positions)
         norm, wd = self._check_weights(q, k, q_weight, k_weight)
         if norm and inverse:
             raise ValueError("inverse takes no norm: see backward")
+        if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad or q_weight is not None
+                                        and (q_weight.requires_grad or k_weight is not None and k_weight.requires_grad)
+                                        or out is not None and any(t is not None and t.requires_grad for t in out)):
+            if out is not None:
+                raise ValueError("out: an input or output requires a gradient")
+            return _Turned.apply(self, q, k, positions, q_weight, k_weight, eps, inverse)
+        positions = checked
         qo, ko = self._outputs(q, k, out)
+        if out is not None:
+            increment_version([t for t in out if t is not None])
         if B * N == 0 or q.shape[-2] == 0:
             return qo, ko
         Hk = 0 if k is None else k.shape[-2]
@@ -210,7 +244,7 @@ class Rotary:
     def backward(self, dq, dk, positions, *, q=None, k=None, q_weight=None, k_weight=None, eps=1e-6, out=None):
         """Gradients of the inputs from those of the outputs: (dq, dk, dq_weight, dk_weight), the last two in fp32 and None
         without a norm.  With a norm q and k are the inputs of the call.  out: (dq, dk) to write to, which may be the
-        gradients that are read."""
+        gradients that are read.  What autograd runs; for those who keep their own inputs."""
         if q_weight is None and k_weight is None:
             return (*self(dq, dk, positions, out=out, inverse=True), None, None)
         positions, B, N, pa, pb = self._common(dq, dk, positions)
@@ -224,6 +258,8 @@ class Rotary:
                     raise ValueError(f"{name}: expected {tuple(d.shape)}, got {tuple(t.shape)}")
         norm, wd = self._check_weights(q, k, q_weight, k_weight)
         qo, ko = self._outputs(dq, dk, out)
+        if out is not None:
+            increment_version([t for t in out if t is not None])
         dwq = torch.empty(q_weight.shape[0], dtype=torch.float32, device=self.dev)
         dwk = None if k is None else torch.empty(k_weight.shape[0], dtype=torch.float32, device=self.dev)
         H, Hk, D = q.shape[-2], 0 if k is None else k.shape[-2], self.head_dim
