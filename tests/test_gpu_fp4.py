@@ -695,3 +695,25 @@ def test_modulated_quantize_with_wide_vectors(fmt, dtype, M, K):
             with pytest.raises(ValueError):
                 call()
     check_status()
+
+
+def test_writing_to_out_is_seen_by_autograd():
+    x = torch.randn(5, 64, generator=gen(1)).to(DEV)
+    up, down = (Fp4Linear(torch.randn(n, k, generator=gen(n)).to(DEV)) for n, k in ((96, 64), (64, 96)))
+    square, a = Fp4Linear(torch.randn(64, 64, generator=gen(3)).to(DEV)), fp4_quantize(x)
+    for call in (lambda y: square(x, out=y), lambda y: square(y, out=y), lambda y: Fp4FeedForward(up, down)(x, out=y),
+                 lambda y: fp4_matmul(a, square.w, out=y), lambda y: a.dequantize(out=y)):
+        y, w = torch.ones(5, 64, device=DEV), torch.ones(64, device=DEV, requires_grad=True)
+        loss = (y * w).sum()      # saves y
+        call(y)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    t = Fp4Tensor.empty(5, 64, "nvfp4", device=DEV)
+    for call in (lambda: fp4_quantize(x, out=t), lambda: fp4_matmul(a, square.w, out=t)):
+        before = t.data._version
+        call()
+        assert t.data._version > before
+    with torch.inference_mode():
+        y = x.clone()
+        assert square(y, out=y) is y
+    check_status()

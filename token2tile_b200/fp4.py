@@ -6,7 +6,7 @@
 
 Formats: "mxfp4" (blocks of 32, scale a power of two) and "nvfp4" (blocks of 16, scale an 8-bit float with 3 mantissa bits, and
 one scale for the whole matrix).  Elements are 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives.  The products run on the
-4-bit tensor cores and sum in 32 bits.
+4-bit tensor cores and sum in 32 bits.  No gradients pass through any of these: their results require none.
 """
 from __future__ import annotations
 
@@ -15,6 +15,7 @@ import math
 import threading
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._launch import DTYPES, launch
@@ -146,6 +147,8 @@ class Fp4Tensor:
             out = torch.empty(rows, K, dtype=dtype, device=self.device)
         elif tuple(out.shape) != self.shape or out.dtype not in DTYPES or out.device != self.device or out.stride(1) != 1:
             raise ValueError(f"out: expected [{rows}, {K}] with contiguous rows on {self.device}")
+        else:
+            increment_version(out)
         if rows:
             launch(self.device, "t2t_fp4_dequantize", _lib.load().t2t_fp4_dequantize, *self.pointers(), rows, K, FORMATS[self.fmt],
                    self.tensor_scale, out.data_ptr(), out.stride(0) if rows > 1 else K, DTYPES[out.dtype])
@@ -220,13 +223,16 @@ def fp4_quantize(x, fmt="nvfp4", *, tensor_scale=1.0, shift=None, scale=None, ep
     x = _rows("x", x)
     M, K = x.shape
     kind = _modulation(shift, scale, K, x.device, x.dtype)
-    if out is None:
+    given = out is not None
+    if not given:
         out = Fp4Tensor.empty(M, K, fmt, tensor_scale, x.device)
     elif out.shape != (M, K) or out.fmt != fmt or out.device != x.device:
         raise ValueError(f"out: expected [{M}, {K}] {fmt} on {x.device}, got {out}")
     if not 2.0 ** -100 <= tensor_scale <= 2.0 ** 100 or (fmt == "mxfp4" and tensor_scale != 1):
         raise ValueError(f"tensor_scale: expected 1 (mxfp4) or 2^-100 .. 2^100 (nvfp4), got {tensor_scale}")
     out.tensor_scale = float(tensor_scale)
+    if given:
+        increment_version(out.data)
     if M:
         launch(x.device, "t2t_fp4_quantize", _lib.load().t2t_fp4_quantize, x.data_ptr(), x.stride(0), ptr(shift), ptr(scale), eps, M,
                K, kind, _fmt(fmt), tensor_scale, *out.pointers())
@@ -248,6 +254,7 @@ def fp4_matmul(a, w, *, bias=None, activation=None, gate=None, residual=None, dt
         raise ValueError(f"unknown activation {activation!r}")
     _vector("bias", bias, N, dev)
     _vector("gate", gate, N, dev, None if bias is None else bias.dtype)
+    given = out is not None
     codes = isinstance(out, Fp4Tensor) or (out is None and dtype in FORMATS)
     if codes:
         if residual is not None or (dtype if out is None else out.fmt) != a.fmt:
@@ -264,6 +271,8 @@ def fp4_matmul(a, w, *, bias=None, activation=None, gate=None, residual=None, dt
         if t is not None and (tuple(t.shape) != (M, N) or t.device != dev or not codes and (
                 t.dtype != out.dtype or t.dtype not in DTYPES or (t.stride(1) != 1 and N != 1))):
             raise ValueError(f"{name}: expected [{M}, {N}] of the result's type with contiguous rows on {dev}, got {t!r}"[:300])
+    if given:
+        increment_version(out.data if codes else out)
     if M == 0 or N == 0:
         return out
     if residual is not None:
@@ -352,7 +361,11 @@ def _layer(x, K, last, bias, shift, scale, gate, residual, out, activation, ws_b
     for name, t in (("residual", residual), ("out", out)):
         if t is not None and (t.shape != shape or t.dtype != x.dtype or t.device != dev):
             raise ValueError(f"{name}: expected {x.dtype} {shape} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    y = torch.empty(*shape, dtype=x.dtype, device=dev) if out is None else out
+    if out is None:
+        y = torch.empty(*shape, dtype=x.dtype, device=dev)
+    else:
+        y = out
+        increment_version(y)
     M = rows.shape[0]
     if M == 0 or N == 0:
         return rows, kind, 0, y, None, None, None
