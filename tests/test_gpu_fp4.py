@@ -717,3 +717,19 @@ def test_writing_to_out_is_seen_by_autograd():
         y = x.clone()
         assert square(y, out=y) is y
     check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M,N", [(3, 264), (140, 136), (1500, 1672), (1500, 1671)])
+def test_residual_of_one_row_for_all(dtype, M, N):
+    """Broadcast over the rows (stride 0), or rows that overlap: the same bits as written out."""
+    a, w = stored(M, 96, "nvfp4", 1), stored(N, 96, "nvfp4", 2)
+    row = torch.randn(1, N, generator=gen(3)).to(dtype).to(DEV)
+    for residual in (row.expand(M, N), torch.randn(8 * M + N, generator=gen(4)).to(dtype).to(DEV).as_strided((M, N), (8, 1))):
+        want = fp4_matmul(a, w, residual=residual.contiguous(), dtype=dtype)
+        assert torch.equal(fp4_matmul(a, w, residual=residual, dtype=dtype), want)
+        out = torch.empty_like(want)
+        assert torch.equal(fp4_matmul(a, w, residual=residual, out=out), want)
+    layer, x = Fp4Linear(w), torch.randn(M, 96, generator=gen(5)).to(dtype).to(DEV)
+    assert torch.equal(layer(x, residual=row.expand(M, N)), layer(x, residual=row.repeat(M, 1)))
+    check_status()

@@ -55,8 +55,8 @@ constexpr int MM_TILE = 256;                       // rows and columns of a pair
 constexpr int MM_K = 256;                          // codes of K a stage: 128 bytes a row
 constexpr int MM_STAGES = 5;
 constexpr int MM_HALF = 128 * 128;                 // bytes of 128 rows of codes
-// How a pair's results leave: MM_TMA by tiles of 128 rows x 128 bytes, where rows are 16-byte aligned; MM_LANES by element, where they
-// are not; MM_CODES quantised.
+// How a pair's results leave: MM_TMA by tiles of 128 rows x 128 bytes, where rows are 16-byte aligned and residuals' rows apart; MM_LANES
+// by element, where they are not; MM_CODES quantised.
 enum MmEpilogue { MM_TMA, MM_LANES, MM_CODES };
 __host__ __device__ constexpr int mm_warps(MmEpilogue e) { return e == MM_TMA ? 8 : 16; }
 __host__ __device__ constexpr int mm_threads(MmEpilogue e) { return 32 * (2 + mm_warps(e)); }
@@ -885,7 +885,8 @@ static int mm_launch(MmMaps& maps, const MmArgs& p, const MmPlan& plan, cudaStre
   if constexpr (std::is_same<T, uint8_t>::value) {
     return mm_launch_pairs<FMT, T, MM_CODES>(maps, p, st);
   } else {
-    if (!p.wide) return mm_launch_pairs<FMT, T, MM_LANES>(maps, p, st);
+    // rows of a residual that overlap (one row for all: stride 0) are no tensor that TMA describes
+    if (!p.wide || (p.residual && p.res_row < p.N)) return mm_launch_pairs<FMT, T, MM_LANES>(maps, p, st);
     if (!mm_result_maps<T>(maps, p)) return T2T_ERR_CUDA;
     return mm_launch_pairs<FMT, T, MM_TMA>(maps, p, st);
   }
