@@ -91,3 +91,10 @@ def test_gradient_formula_against_differences(layout, norm):
         d = torch.zeros_like(w)
         d[i] = h
         assert abs(float((f(x, w + d) - f(x, w - d)) / (2 * h) - dw[i])) < 1e-8
+
+
+def test_yarn_attention_factor():
+    """0.1 ln(factor) + 1 for stretched contexts, 1 where nothing is stretched, or as given."""
+    of = lambda factor, **kw: rotary_frequencies(64, scaling=dict(type="yarn", factor=factor, original_length=4096, **kw))[1]
+    assert math.isclose(of(8.0), 0.1 * math.log(8.0) + 1) and of(1.0) == of(0.5) == of(0.01) == 1.0
+    assert of(0.5, attention_factor=0.7) == 0.7

@@ -31,7 +31,7 @@ def rotary_frequencies(width, base=10000.0, scaling=None):
       ntk      the base multiplied by factor^(width / (width - 2)): the fastest pair stays, the slowest is divided by the factor
       yarn     pairs that turn more than `beta_fast` (32) times within `original_length` positions stay, those below `beta_slow`
                (1) turns are divided by the factor, a linear ramp over the pair's number in between; cosine and sine
-               multiplied by `attention_factor` (0.1 ln(factor) + 1)
+               multiplied by `attention_factor` (0.1 ln(factor) + 1, and 1 for factors below 1)
       bands    the same by wavelength: below original_length / `high_factor` (4) stay, above original_length / `low_factor` (1)
                divided, in between mixed linearly in the reciprocal of the wavelength
     """
@@ -58,7 +58,7 @@ def rotary_frequencies(width, base=10000.0, scaling=None):
             pair = lambda turns: width * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
             low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), width - 1)
             kept = [1.0 - min(max((j - low) / max(high - low, 1e-3), 0.0), 1.0) for j in range(width // 2)]
-            mscale = float(s.pop("attention_factor", 0.1 * math.log(factor) + 1.0))
+            mscale = float(s.pop("attention_factor", 0.1 * math.log(max(factor, 1.0)) + 1.0))
         else:
             lo, hi = float(s.pop("low_factor", 1.0)), float(s.pop("high_factor", 4.0))
             if not hi > lo:
