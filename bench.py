@@ -600,6 +600,15 @@ def dit_roofline(linear, gemm_flops, ms_step, pk):
             "note": note + (f"; peak derived: 4 x the {pk['src']} sustained bf16 rate" if linear else "")}
 
 
+def check_waits(dev, linear, runtimes):
+    """Raises if a bounded wait of the step's kernels gave up: the times would be those of wrong results."""
+    for rt in runtimes:
+        assert rt.deploy.device_status() == 0, "a device wait timed out"
+    if linear:
+        from token2tile_b200.fp4 import check_status
+        check_status(dev)
+
+
 def dit_measure(rank, world, dev, group, *, grid_name="720p", blocks=0, dense_attention=False, steps=4, warmup=4,
                 with_e2e=True, linear=None):
     """One denoising step = both CFG branches through all blocks.  The timed steps cover whole refresh periods
@@ -707,9 +716,7 @@ def dit_measure(rank, world, dev, group, *, grid_name="720p", blocks=0, dense_at
         counter[0] = (counter[0] + 3) // 4 * 4
         e2e_ms = maxr(time_events(lambda: denoise_step(host=True), steps) / steps)
         barrier()
-    if not dense_attention:
-        for rt in B._RUNTIMES.values():
-            assert rt.deploy.device_status() == 0, "a device wait timed out"
+    check_waits(dev, linear, [] if dense_attention else B._RUNTIMES.values())
     line = None
     if rank == 0:
         pk = peaks()
