@@ -331,3 +331,24 @@ def test_writing_to_out_is_seen_by_autograd():
     with torch.inference_mode():
         x, y = q.clone(), k.clone()
         assert rot(x, y, pos, out=(x, y))[0] is x
+
+
+@pytest.mark.parametrize("norm", ["", "head", "row"])
+def test_no_heads_of_queries(norm):
+    """k is turned all the same."""
+    gen = torch.Generator().manual_seed(14)
+    rot = Rotary(64)
+    pos = torch.arange(7, device=DEV) + 3
+    k, dk = make((7, 3, 64), F32, gen, False, 3)
+    q = torch.empty(7, 0, 64, device=DEV)
+    n = dict(head=64, row=3 * 64).get(norm)
+    w = None if n is None else 1 + 0.2 * torch.randn(n, generator=gen).to(DEV)
+    wq = None if n is None else torch.ones(64 if norm == "head" else 0, device=DEV)
+    out = torch.full_like(k, 7.0)
+    got = rot(q, k, pos, q_weight=wq, k_weight=w, out=(q, out))
+    assert got[0] is q and got[1] is out and torch.equal(out, rot(k, None, pos, q_weight=w)[0])
+    back = rot.backward(q, dk, pos, q=q, k=k, q_weight=wq, k_weight=w)
+    want = rot.backward(dk, None, pos, q=k, q_weight=w)
+    assert back[0].shape == q.shape and torch.equal(back[1], want[0])
+    if norm:
+        assert not bool(back[2].any()) and torch.equal(back[3], want[2])

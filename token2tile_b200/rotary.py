@@ -231,7 +231,11 @@ class Rotary:
         qo, ko = self._outputs(q, k, out)
         if out is not None:
             increment_version([t for t in out if t is not None])
-        if B * N == 0 or q.shape[-2] == 0:
+        if B * N == 0:
+            return qo, ko
+        if q.shape[-2] == 0:      # k alone
+            if k is not None:
+                self(k, None, positions, q_weight=k_weight, eps=eps, out=(ko, None), inverse=inverse)
             return qo, ko
         Hk = 0 if k is None else k.shape[-2]
         kk, kko = (k, ko) if Hk else (q, qo)
@@ -263,6 +267,9 @@ class Rotary:
         dwq = torch.empty(q_weight.shape[0], dtype=torch.float32, device=self.dev)
         dwk = None if k is None else torch.empty(k_weight.shape[0], dtype=torch.float32, device=self.dev)
         H, Hk, D = q.shape[-2], 0 if k is None else k.shape[-2], self.head_dim
+        if H == 0 and Hk and B * N:
+            ko, _, dwk, _ = self.backward(dk, None, positions, q=k, q_weight=k_weight, eps=eps, out=(ko, None))
+            return qo, ko, dwq.zero_(), dwk
         if B * N == 0 or H == 0:
             return qo, ko, dwq.zero_(), None if dwk is None else dwk.zero_()
         side_k = (k, dk, ko) if Hk else (q, dq, qo)
