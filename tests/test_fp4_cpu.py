@@ -166,3 +166,15 @@ def test_a_device_has_one_status_word(monkeypatch):
     for t in threads:
         t.join()
     assert len(got) == 8 and all(s is fp4._status[i] for i, s in got) and fp4._status[0] is not fp4._status[1]
+
+
+def test_refuses_matrices_on_the_host():
+    import pytest
+
+    from token2tile_b200 import Fp4FeedForward, Fp4Linear, fp4_matmul
+    a, w = Fp4Tensor.empty(3, 64, "nvfp4", device="cpu"), Fp4Tensor.empty(64, 64, "nvfp4", device="cpu")
+    x, layer = torch.zeros(3, 64), Fp4Linear(w)
+    for call in (a.dequantize, lambda: fp4_matmul(a, w), lambda: fp4_matmul(a, w, dtype="nvfp4"), lambda: layer(a), lambda: layer(x),
+                 lambda: Fp4FeedForward(layer, layer)(x)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()

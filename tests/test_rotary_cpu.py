@@ -98,3 +98,13 @@ def test_yarn_attention_factor():
     of = lambda factor, **kw: rotary_frequencies(64, scaling=dict(type="yarn", factor=factor, original_length=4096, **kw))[1]
     assert math.isclose(of(8.0), 0.1 * math.log(8.0) + 1) and of(1.0) == of(0.5) == of(0.01) == 1.0
     assert of(0.5, attention_factor=0.7) == 0.7
+
+
+def test_refuses_tensors_on_the_host():
+    """A plan made on the host has the host's tensors pass as its own; their pointers never reach a kernel."""
+    rot = Rotary(8, device="cpu")
+    q, pos, w = torch.zeros(2, 3, 8), torch.arange(2), torch.ones(8)
+    for call in (lambda: rot(q, None, pos), lambda: rot(q, q, pos, q_weight=w, k_weight=w), lambda: rot.backward(q, None, pos),
+                 lambda: rot.backward(q, q, pos, q=q, k=q, q_weight=w, k_weight=w)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()

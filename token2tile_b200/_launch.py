@@ -19,6 +19,8 @@ if _raw_stream is None or _current_device is None:
 def launch(dev, what, fn, *args):
     """fn(*args, stream) on the current stream of the CUDA device `dev`; raises RuntimeError for an error code."""
     index = dev.index
+    if index is None:      # a tensor's CUDA device has one
+        raise ValueError(f"{what}: expected tensors on a CUDA device, got {dev}")
     if _current_device() == index:
         code = fn(*args, _raw_stream(index))
     else:

@@ -44,6 +44,8 @@ _status_lock = threading.Lock()      # queued kernels point to the word: a devic
 def _status_of(dev):
     s = _status.get(dev.index)
     if s is None:
+        if dev.index is None:
+            raise ValueError(f"expected tensors on a CUDA device, got {dev}")
         with _status_lock:
             s = _status.get(dev.index)
             if s is None:
