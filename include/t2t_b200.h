@@ -349,7 +349,7 @@ int t2t_fp4_dequantize(const void* codes, const void* scales, int M, int K, int 
                        long long out_row_stride, int dtype, cudaStream_t stream);
 
 /* out[m, n] = residual[m, n] + gate[n] * act(alpha * sum_k A[m, k] W[n, k] + bias[n]) of 4-bit matrices A [M, K] and
- * W [N, K] of one format; alpha holds the tensor scales.  Sums in 32 bits, one rounding.  bias, gate [N] (NULL: none) of type
+ * W [N, K] of one format; alpha, finite, holds the tensor scales.  Sums in 32 bits, one rounding.  bias, gate [N] (NULL: none) of type
  * vec_dtype, residual [M, N] (NULL: none; row stride 0: one row for all) and out of type dtype; out may be residual (same address and row stride) and overlaps
  * no other input: T2T_ERR_ARG for a factor, not checked for the rest. */
 int t2t_fp4_matmul(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, int M, int N, int K,

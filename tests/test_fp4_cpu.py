@@ -178,3 +178,15 @@ def test_refuses_matrices_on_the_host():
                  lambda: Fp4FeedForward(layer, layer)(x)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_tensor_scales_whose_product_has_no_32_bits(lib):
+    import pytest
+
+    from token2tile_b200 import fp4_matmul
+    x = 4096                     # never read
+    for alpha in (math.inf, -math.inf, math.nan):
+        assert lib.t2t_fp4_matmul(x, 2 * x, 3 * x, 4 * x, 4, 8, 64, 1, alpha, 0, 0, 0, 0, 0, 0, 5 * x, 8, 0, 0, 0) == 1
+    a, w = (Fp4Tensor.empty(3, 64, "nvfp4", g, device="cpu") for g in (2.0 ** 100, 2.0 ** 28))
+    with pytest.raises(ValueError, match="32 bits"):
+        fp4_matmul(a, w)

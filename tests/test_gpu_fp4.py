@@ -733,3 +733,16 @@ def test_residual_of_one_row_for_all(dtype, M, N):
     layer, x = Fp4Linear(w), torch.randn(M, 96, generator=gen(5)).to(dtype).to(DEV)
     assert torch.equal(layer(x, residual=row.expand(M, N)), layer(x, residual=row.repeat(M, 1)))
     check_status()
+
+
+@pytest.mark.parametrize("M", [2, 300])
+def test_largest_tensor_scales(M):
+    """Zeros stay zeros under the largest product of tensor scales that is taken."""
+    a, w = (Fp4Tensor.empty(rows, 64, "nvfp4", g, DEV) for rows, g in ((M, 2.0 ** 100), (40, 2.0 ** 27)))
+    for t in (a, w):
+        t.data.zero_()
+    assert not bool(fp4_matmul(a, w, dtype=F32).any())
+    w.tensor_scale = 2.0 ** 28
+    with pytest.raises(ValueError, match="32 bits"):
+        fp4_matmul(a, w, dtype=F32)
+    check_status()

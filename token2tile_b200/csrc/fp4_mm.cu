@@ -913,6 +913,7 @@ static int mm_run(const void* a_codes, const void* a_scales, const void* w_codes
                   const MmArgs& p, cudaStream_t stream) {
   if ((!p.x && (!a_codes || !a_scales)) || !w_codes || !w_scales || !p.out || p.M <= 0 || p.N <= 0 || p.K <= 0 || p.K > (1 << 24))
     return T2T_ERR_ARG;
+  if (!(p.alpha - p.alpha == 0.f)) return T2T_ERR_ARG;      // an infinity would make NaN of sums that are 0
   if (!fp4_known(fmt) || !elem_known(p.vec_dtype) || p.act < T2T_ACT_NONE || p.act > T2T_ACT_SILU) return T2T_ERR_ARG;
   if (((uintptr_t)a_codes | (uintptr_t)a_scales | (uintptr_t)w_codes | (uintptr_t)w_scales) % 16) return T2T_ERR_ARG;
   if ((long long)cdiv(p.M, MM_TILE) * cdiv(p.N, MM_TILE) > 0x3fffffffLL) return T2T_ERR_ARG;

@@ -247,11 +247,16 @@ def fp4_matmul(a, w, *, bias=None, activation=None, gate=None, residual=None, dt
     result's type; out may be the residual, and shares no memory with the other inputs.
 
     dtype "mxfp4" or "nvfp4" (the format of a and w), or an Fp4Tensor [M, N] as out: the result quantised as by fp4_quantize,
-    from 32 bits; takes no residual."""
+    from 32 bits; takes no residual.
+
+    The tensor scales' product is a factor in 32 bits: one of 2^128 or more is refused, one below 2^-149 is 0."""
     (M, K), (N, Kw) = a.shape, w.shape
     dev = a.device
     if K != Kw or a.fmt != w.fmt or w.device != dev:
         raise ValueError(f"expected matrices of one format, width and device, got {a} and {w}")
+    alpha = a.tensor_scale * w.tensor_scale
+    if alpha >= 2.0 ** 128:
+        raise ValueError(f"tensor scales {a.tensor_scale} and {w.tensor_scale}: their product leaves the range of 32 bits")
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     _vector("bias", bias, N, dev)
@@ -282,7 +287,7 @@ def fp4_matmul(a, w, *, bias=None, activation=None, gate=None, residual=None, dt
     status = _status_of(dev)
     if status.value.value:
         check_status(dev, wait=False)
-    head = (*a.pointers(), *w.pointers(), M, N, K, FORMATS[a.fmt], a.tensor_scale * w.tensor_scale, ptr(bias),
+    head = (*a.pointers(), *w.pointers(), M, N, K, FORMATS[a.fmt], alpha, ptr(bias),
             ACTIVATIONS[activation], ptr(gate), _vector_type(bias, gate))
     if codes:
         launch(dev, "t2t_fp4_matmul_quantize", _lib.load().t2t_fp4_matmul_quantize, *head, out.tensor_scale, *out.pointers(),
