@@ -352,3 +352,66 @@ def test_no_heads_of_queries(norm):
     assert back[0].shape == q.shape and torch.equal(back[1], want[0])
     if norm:
         assert not bool(back[2].any()) and torch.equal(back[3], want[2])
+
+
+@pytest.mark.parametrize("axes", [None, (24, 20, 20)])
+@pytest.mark.parametrize("norm", ["", "row"])
+def test_positions_shared_over_a_batch(axes, norm):
+    """[N] or [A, N] for q [B, N, H, D], also as expanded, transposed and 32-bit views: as the sequences one by one."""
+    gen = torch.Generator().manual_seed(15)
+    rot = Rotary(64, layout="half", axes=axes)
+    q, k = make((3, 11, 4, 64), BF, gen, True, 2)
+    dq, dk = make((3, 11, 4, 64), BF, gen, False, 2)
+    pos = (torch.randint(0, 5000, (11,) if axes is None else (3, 11), generator=gen)).to(DEV)
+    w = (None, None) if not norm else tuple((1 + 0.2 * torch.randn(h * 64, generator=gen)).to(BF).to(DEV) for h in (4, 2))
+    kw = dict(q_weight=w[0], k_weight=w[1])
+    want = [rot(q[b], k[b], pos, **kw) for b in range(3)]
+    grads = [rot.backward(dq[b], dk[b], pos, q=q[b], k=k[b], **kw) for b in range(3)]
+    each = pos.unsqueeze(-2).expand(*pos.shape[:-1], 3, 11)
+    for p in (pos, each, each.contiguous(), pos.to(torch.int32), pos.repeat_interleave(2, -1)[..., ::2]):
+        got, back = rot(q, k, p, **kw), rot.backward(dq, dk, p, q=q, k=k, **kw)
+        for i in range(2):
+            assert torch.equal(got[i], torch.stack([t[i] for t in want])) and torch.equal(back[i], torch.stack([t[i] for t in grads]))
+
+
+@pytest.mark.parametrize("dtype,D,rd", [(BF, 128, 128), (F16, 128, 64), (F32, 128, 128), (BF, 80, 40)])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("norm", ["", "head", "row"])
+def test_addresses_that_are_not_whole_vectors(dtype, D, rd, layout, norm):
+    """q, k, their gradients, results and weights at odd elements and odd strides, one at a time and all: what aligned copies give, but for
+    the order of the norm's sums."""
+    gen = torch.Generator().manual_seed(16)
+    rot = Rotary(D, rd, layout=layout)
+    N, H, Hk = 70, 5, 3
+    pos = torch.arange(N, device=DEV) + 17
+    q, k = make((N, H, D), dtype, gen, False, Hk)
+    dq, dk = make((N, H, D), dtype, gen, False, Hk)
+    w = [None, None] if not norm else [(1 + 0.2 * torch.randn(h * D if norm == "row" else D, generator=gen)).to(dtype).to(DEV) for h in (H, Hk)]
+    off = {"x": (q, k), "dy": (dq, dk), "w": w}
+
+    def odd(t, by):      # the same values `by` elements behind an aligned address, rows an odd number of elements apart
+        if t is None:
+            return None
+        if t.dim() == 1:
+            base = torch.empty(len(t) + by, dtype=t.dtype, device=DEV)
+            base[by:] = t
+            return base[by:]
+        n, h, d = t.shape
+        base = torch.empty(by + n * (h * (d + 1) + 1), dtype=t.dtype, device=DEV)
+        view = base[by:].as_strided((n, h, d), (h * (d + 1) + 1, d + 1, 1), by)
+        return view.copy_(t)
+
+    args, weights = (pos[None].cpu(), rot.frequencies, axis_of(rot)), [None if t is None else t.cpu() for t in w]
+    exact = [plain64.rotary(t.double().cpu(), v, 1e-6, *args, layout=layout) for t, v in zip((q, k), weights)]
+    exact_grad = [plain64.rotary_grad(d.double().cpu(), t.double().cpu(), v, 1e-6, *args, layout=layout)[0]
+                  for d, t, v in zip((dq, dk), (q, k), weights)]
+    for by in (1, 3):
+        for which in ("x", "dy", "w", "out", "all"):
+            use = {n: [odd(t, by) if which in (n, "all") else t for t in ts] for n, ts in off.items()}
+            out = tuple(odd(t, by) if which in ("out", "all") else torch.empty_like(t) for t in (q, k))
+            got = rot(*use["x"], pos, q_weight=use["w"][0], k_weight=use["w"][1], out=out)
+            for g, e in zip(got, exact):
+                close(g, e, dtype)
+            back = rot.backward(*use["dy"], pos, q=use["x"][0], k=use["x"][1], q_weight=use["w"][0], k_weight=use["w"][1], out=out)
+            for g, e in zip(back, exact_grad):
+                close(g, e, dtype)
