@@ -180,9 +180,7 @@ def _vector(name, v, n, dev, dtype=None):
 
 
 def _modulation(shift, scale, K, dev, dtype):
-    """Checks of shift and scale; the C entries' type of an x of `dtype` with them."""
-    if shift is None and scale is None:
-        return DTYPES[dtype]
+    """Checks of shift and scale, of which there is one; the C entries' type of an x of `dtype` with them."""
     if shift is None or scale is None:
         raise ValueError("shift and scale are given together")
     kind = torch.float32 if shift.dtype == torch.float32 else dtype
@@ -224,7 +222,7 @@ def fp4_quantize(x, fmt="nvfp4", *, tensor_scale=1.0, shift=None, scale=None, ep
     weight w as scale = w - 1 is given in float32: in 16 bits the difference loses what w has below 2^-8.)"""
     x = _rows("x", x)
     M, K = x.shape
-    kind = _modulation(shift, scale, K, x.device, x.dtype)
+    kind = DTYPES[x.dtype] if shift is None and scale is None else _modulation(shift, scale, K, x.device, x.dtype)
     given = out is not None
     if not given:
         out = Fp4Tensor.empty(M, K, fmt, tensor_scale, x.device)
@@ -363,7 +361,7 @@ def _layer(x, K, last, bias, shift, scale, gate, residual, out, activation, ws_b
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     rows = _rows("x", x)
-    kind = _modulation(shift, scale, K, dev, x.dtype)
+    kind = DTYPES[x.dtype] if shift is None and scale is None else _modulation(shift, scale, K, dev, x.dtype)
     _vector("gate", gate, N, dev, None if bias is None else bias.dtype)
     for name, t in (("residual", residual), ("out", out)):
         if t is not None and (t.shape != shape or t.dtype != x.dtype or t.device != dev):

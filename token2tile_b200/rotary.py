@@ -221,9 +221,9 @@ class Rotary:
         norm, wd = self._check_weights(q, k, q_weight, k_weight)
         if norm and inverse:
             raise ValueError("inverse takes no norm: see backward")
-        if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad or q_weight is not None
-                                        and (q_weight.requires_grad or k_weight is not None and k_weight.requires_grad)
-                                        or out is not None and any(t is not None and t.requires_grad for t in out)):
+        if (q.requires_grad or k is not None and k.requires_grad or q_weight is not None
+                and (q_weight.requires_grad or k_weight is not None and k_weight.requires_grad)
+                or out is not None and any(t is not None and t.requires_grad for t in out)) and torch.is_grad_enabled():
             if out is not None:
                 raise ValueError("out: an input or output requires a gradient")
             return _Turned.apply(self, q, k, positions, q_weight, k_weight, eps, inverse)
