@@ -119,20 +119,16 @@ __device__ __forceinline__ void tma_load_tile3_pair(uint32_t dst, const void* ma
 // tanh(u) = 2 / (1 + exp(-2 u)) - 1, so both activations are x / (1 + 2^-z).  ex2 and rcp are good to 2^-22; z, of a few
 // tens at most where the result is not x or 0, adds 2^-20 at worst.  Large arguments: z overflows to an infinity of the right sign
 // and the result is x or -0.  GELU's x^2 may overflow in it; SiLU has no such term (times a factor of 0 it would be a NaN).
-template <int n>
-__device__ __forceinline__ void mm_act(float (&y)[n], int act) {
-  if (act == T2T_ACT_NONE) return;
-  constexpr float log2e = 1.4426950408889634f;
-  const float c1 = act == T2T_ACT_SILU ? -log2e : -1.5957691216057308f * log2e;
-  constexpr float c3 = 0.044715f * -1.5957691216057308f * log2e;
+template <int ACT, int n>
+__device__ __forceinline__ void mm_act_of(float (&y)[n]) {
+  constexpr float log2e = 1.4426950408889634f, c1 = ACT == T2T_ACT_SILU ? -log2e : -1.5957691216057308f * log2e,
+                  c3 = 0.044715f * -1.5957691216057308f * log2e;
   const uint64_t k1 = pair_of(c1, c1), k3 = pair_of(c3, c3), one = pair_of(1.f, 1.f);
 #pragma unroll
   for (int e = 0; e < n; e += 2) {
     const uint64_t x = pair_of(y[e], y[e + 1]);
     float p, q;
-    uint64_t z = k1;
-    if (act == T2T_ACT_GELU_TANH) z = fma2(k3, mul2(x, x), k1);
-    pair_to(mul2(x, z), p, q);
+    pair_to(mul2(x, ACT == T2T_ACT_SILU ? k1 : fma2(k3, mul2(x, x), k1)), p, q);
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(q));
     pair_to(add2(pair_of(p, q), one), p, q);
@@ -140,6 +136,11 @@ __device__ __forceinline__ void mm_act(float (&y)[n], int act) {
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(q));
     pair_to(mul2(x, pair_of(p, q)), y[e], y[e + 1]);
   }
+}
+template <int n>
+__device__ __forceinline__ void mm_act(float (&y)[n], int act) {
+  if (act == T2T_ACT_GELU_TANH) mm_act_of<T2T_ACT_GELU_TANH>(y);
+  else if (act == T2T_ACT_SILU) mm_act_of<T2T_ACT_SILU>(y);
 }
 // y * a + b, by pairs.
 template <int n>
