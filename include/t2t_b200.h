@@ -305,7 +305,7 @@ int t2t_rotation_selftest(const double* d_pairs, double* d_out, int n, cudaStrea
 /* Rotary positions of q [batch, N, Hq, D] and k [batch, N, Hk, D] (Hk = 0: q alone).  Pair j < rotary_dim / 2 of every
  * head, elements (2 j, 2 j + 1) if `interleaved` and (j, j + rotary_dim / 2) otherwise, is turned by
  * theta = position[axis[j]] * f_j (by -theta if `inverse`, which is the gradient) and multiplied by mscale; the other
- * elements pass.  turns[j]: f_j / (2 pi) modulo 1 in units of 2^-64, so that theta is right at any position.
+ * elements pass.  turns[j]: f_j / (2 pi) modulo 1 in units of 2^-64; theta is off by position times its error.
  * positions: int32 or int64 (pos_bytes), token n of batch b and axis a at a * pos_axis_stride + b * pos_batch_stride + n.
  * norm: RMS norm in front, over a head (weights [D]) or over the row of all heads (weights [Hq * D] and [Hk * D]), its
  * weights of the type of q and k or 32 bits (weight_dtype); not with `inverse`.  strides, on the host, in elements:

@@ -108,3 +108,16 @@ def test_refuses_tensors_on_the_host():
                  lambda: rot.backward(q, q, pos, q=q, k=q, q_weight=w, k_weight=w)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_error_of_the_frequencies():
+    """The frequencies are 64-bit floats, turned into turns in 64-bit floats: within 2^-55 turns a position of the exact f / (2 pi), which is
+    what limits the angle far out (behind 2^29 positions it is more than the rounding to 32 bits).  That whole turns drop out
+    exactly says nothing about this."""
+    from fractions import Fraction
+    pi = Fraction(31415926535897932384626433832795028841971693993751058209749445923, 10 ** 64)
+    for width, base in ((8, 1e4), (64, 1e4), (128, 5e5), (128, 1e6), (256, 1e4), (512, 1e4)):
+        rot = Rotary(width, base=base, device="cpu")
+        for t, f in zip(rot.turns.tolist(), rot.frequencies):
+            off = abs(Fraction(t % 2 ** 64, 2 ** 64) - Fraction(f) / (2 * pi))
+            assert off <= Fraction(1, 2 ** 55)

@@ -5,8 +5,8 @@
 //
 // on the pairs (2 j, 2 j + 1) or (j, j + rotary_dim / 2) of every head; the rest of the head passes unchanged.  The
 // frequencies come as turns per position in units of 2^-64: the 64-bit product with the position drops whole turns
-// without rounding, so the angle is right to 32 bits at any position (position * f in 32 bits is off by 0.008 rad at
-// 131,072).  Statistics, angles and the rotation are held in 32 bits; each output is rounded once.
+// without rounding, so what is off is the position times the error of the frequency itself.  Rotary's, out of 64-bit floats, are right to
+// 2^-55 turns, and the angle to 32 bits up to 2^29 positions (position * f in 32 bits is off by 0.008 rad at 131,072).  Statistics, angles and the rotation are held in 32 bits; each output is rounded once.
 //
 // An item is two vectors of V elements that hold V pairs.  L lanes (a power of two) work on one head of one token, a
 // block on all heads of q and k of one token: the cosines are computed once per token and shared by all heads.
