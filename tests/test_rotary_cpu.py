@@ -121,3 +121,13 @@ def test_error_of_the_frequencies():
         for t, f in zip(rot.turns.tolist(), rot.frequencies):
             off = abs(Fraction(t % 2 ** 64, 2 ** 64) - Fraction(f) / (2 * pi))
             assert off <= Fraction(1, 2 ** 55)
+
+
+def test_refusals_of_scalings():
+    for kind in ("yarn", "bands"):
+        for kw in (dict(), dict(original_length=0), dict(original_length=-4096)):
+            with pytest.raises(ValueError, match="original_length"):
+                rotary_frequencies(64, scaling=dict(type=kind, factor=2.0, **kw))
+    with pytest.raises(ValueError, match="base"):
+        rotary_frequencies(64, 1.0, scaling=dict(type="yarn", factor=2.0, original_length=4096))
+    assert rotary_frequencies(64, 1.0)[0] == [1.0] * 32

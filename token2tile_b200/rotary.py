@@ -52,7 +52,11 @@ def rotary_frequencies(width, base=10000.0, scaling=None):
     elif kind == "linear":
         freqs = [f / factor for f in freqs]
     elif kind in ("yarn", "bands"):
-        length = float(s.pop("original_length"))
+        length = float(s.pop("original_length", 0.0))
+        if not length > 0:
+            raise ValueError(f"{kind} takes the original_length of the context, got {length}")
+        if kind == "yarn" and base == 1:
+            raise ValueError("yarn takes a base other than 1: its pairs would all have one wavelength")
         if kind == "yarn":
             fast, slow = float(s.pop("beta_fast", 32.0)), float(s.pop("beta_slow", 1.0))
             pair = lambda turns: width * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
