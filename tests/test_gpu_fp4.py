@@ -746,3 +746,17 @@ def test_largest_tensor_scales(M):
     with pytest.raises(ValueError, match="32 bits"):
         fp4_matmul(a, w, dtype=F32)
     check_status()
+
+
+def test_one_column():
+    """Its stride means nothing, in any of the calls."""
+    column = torch.randn(5, 8, generator=gen(1)).to(DEV)[:, ::4][:, :1]
+    assert column.stride() == (8, 4)
+    t = fp4_quantize(column)
+    check_quantized(t, column)
+    out = torch.zeros(5, 8, device=DEV)
+    assert torch.equal(t.dequantize(out=out[:, ::4][:, :1]), t.dequantize()) and not bool(out[:, 1:].any())
+    a, w = stored(5, 64, "nvfp4", 1), stored(1, 64, "nvfp4", 2)
+    want = fp4_matmul(a, w, residual=column, dtype=F32)
+    assert torch.equal(fp4_matmul(a, w, residual=column, out=out[:, ::4][:, :1]), want)
+    check_status()

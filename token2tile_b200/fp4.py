@@ -147,7 +147,8 @@ class Fp4Tensor:
             if dtype not in DTYPES:
                 raise ValueError(f"dtype: expected bfloat16, float16 or float32, got {dtype}")
             out = torch.empty(rows, K, dtype=dtype, device=self.device)
-        elif tuple(out.shape) != self.shape or out.dtype not in DTYPES or out.device != self.device or out.stride(1) != 1:
+        elif tuple(out.shape) != self.shape or out.dtype not in DTYPES or out.device != self.device \
+                or (out.stride(1) != 1 and K != 1):
             raise ValueError(f"out: expected [{rows}, {K}] with contiguous rows on {self.device}")
         else:
             increment_version(out)
