@@ -309,7 +309,7 @@ int t2t_rotation_selftest(const double* d_pairs, double* d_out, int n, cudaStrea
  * positions: int32 or int64 (pos_bytes), token n of batch b and axis a at a * pos_axis_stride + b * pos_batch_stride + n.
  * norm: RMS norm in front, over a head (weights [D]) or over the row of all heads (weights [Hq * D] and [Hk * D]), its
  * weights of the type of q and k or 32 bits (weight_dtype); not with `inverse`.  strides, on the host, in elements:
- * (batch, token, head) of q, k, q_out, k_out.  Outputs may be the inputs.  D and rotary_dim even, rotary_dim <= 512;
+ * (batch, token, head) of q, k, q_out, k_out.  Outputs may be the inputs and overlap them nowhere else.  D and rotary_dim even, rotary_dim <= 512;
  * elements of a head contiguous.  No counterpart in the reference, which leaves positions to its host. */
 int t2t_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight, const void* k_weight,
                int weight_dtype, const void* positions, int pos_bytes, long long pos_axis_stride,

@@ -760,3 +760,19 @@ def test_one_column():
     want = fp4_matmul(a, w, residual=column, dtype=F32)
     assert torch.equal(fp4_matmul(a, w, residual=column, out=out[:, ::4][:, :1]), want)
     check_status()
+
+
+def test_range_of_a_layer():
+    """A layer's own quantisation of nvfp4 holds magnitudes of 0.006 to 2,688; other rows are given quantised with their scale.  The weight, 6
+    on its diagonal, is quantised exactly."""
+    layer = Fp4Linear((6 * torch.eye(64)).to(BF).to(DEV))
+    assert torch.equal(layer.w.dequantize(), 6 * torch.eye(64, device=DEV))
+    row = lambda v: torch.full((5, 64), v, dtype=F32, device=DEV)
+    held = lambda x, **kw: layer(x, **kw) / 6
+    assert not bool(held(row(0.0058)).any()) and bool((held(row(0.006)) > 0.005).all())
+    assert torch.equal(held(row(5000.0)), held(row(2688.0))) and bool((held(row(2688.0)) == 2688.0).all())
+    for v in (1e-6, 3e5):
+        g = fp4_tensor_scale(row(v))
+        got = held(fp4_quantize(row(v), tensor_scale=g), dtype=F32)
+        assert bool(((got / v - 1).abs() < 0.07).all())      # a scale has three bits behind its first
+    check_status()

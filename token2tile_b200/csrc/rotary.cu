@@ -507,8 +507,8 @@ __device__ __forceinline__ void meet(F& v, F* red) {
 
 // Blocks take tokens in turn, with x of the next two on its way.  One meeting of the block a token: behind it the sums of the norm and
 // the angles of this token (computed one token ahead, in the third of three tables) are there.
-// Bound by memory: q and k of 75,600 tokens of 40 heads of 128, 3.1 GB, take 604 us with the norm over all heads and 527
-// without (5.1 and 5.9 TB/s).  One block a token with x loaded to registers took 715; the kernel below, which reads x twice
+// Bound by memory: q and k of 75,600 tokens of 40 heads of 128, 3.1 GB, take 600 us with the norm over all heads and 530
+// without in a loop over the same tensors (5.2 and 5.8 TB/s), 617 to 639 with the norm where they change from call to call.  One block a token with x loaded to registers took 715; the kernel below, which reads x twice
 // and weights one by one, 1,690.
 constexpr int ROT_AHEAD = 3;
 constexpr int fwd_threads(int R) { return R == 4 ? 512 : 256; }

@@ -307,7 +307,11 @@ def fp4_tensor_scale(x):
 
 
 class Fp4Linear:
-    """y = activation(x W^T + b) with W [out, in] quantised once and every x on the way in; plain tensors, no autograd."""
+    """y = activation(x W^T + b) with W [out, in] quantised once and every x on the way in; plain tensors, no autograd.
+
+    x is quantised with a tensor scale of 1: "nvfp4" holds blocks whose largest magnitude is between 0.006 and 2,688 (below 0.1 with
+    fewer bits of scale), saturates above and gives zeros below.  Rows beyond that are quantised by fp4_quantize with a tensor_scale
+    of their own and given so."""
 
     def __init__(self, weight, bias=None, *, fmt="nvfp4"):
         if isinstance(weight, Fp4Tensor):
@@ -386,7 +390,8 @@ def _layer(x, K, last, bias, shift, scale, gate, residual, out, activation, ws_b
 
 class Fp4FeedForward:
     """residual + gate * down(activation(up(layer_norm(x) * (1 + scale) + shift))).  What lies between the two products is
-    quantised from 32 bits, without a rounding to 16 in between."""
+    quantised from 32 bits, without a rounding to 16 in between, and with a tensor scale of 1 as x is (Fp4Linear); hidden values beyond
+    its range go through fp4_matmul into an Fp4Tensor with a scale of their own."""
 
     def __init__(self, up, down, activation="gelu_tanh"):
         if up.w.shape[0] != down.w.shape[1] or up.w.fmt != down.w.fmt or up.w.device != down.w.device:
