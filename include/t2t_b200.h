@@ -302,15 +302,16 @@ int t2t_register_split_selftest(int regs);
  * projection fit's Jacobi rounds turn them by.  No counterpart in the reference. */
 int t2t_rotation_selftest(const double* d_pairs, double* d_out, int n, cudaStream_t stream);
 
-/* Rotary positions of q [batch, N, Hq, D] and k [batch, N, Hk, D] (Hk = 0: q alone).  Pair j < rotary_dim / 2 of every
- * head, elements (2 j, 2 j + 1) if `interleaved` and (j, j + rotary_dim / 2) otherwise, is turned by
- * theta = position[axis[j]] * f_j (by -theta if `inverse`, which is the gradient) and multiplied by mscale; the other
+/* Rotary positions of q [batch, N, Hq, D] and k [batch, N, Hk, D] (Hk = 0: q alone).  Pair j < rotary_dim / 2 of
+ * every head, elements (2 j, 2 j + 1) if `interleaved` and (j, j + rotary_dim / 2) otherwise, is turned by theta =
+ * position[axis[j]] * f_j (by -theta if `inverse`, which is the gradient) and multiplied by mscale; the other
  * elements pass.  turns[j]: f_j / (2 pi) modulo 1 in units of 2^-64; theta is off by position times its error.
- * positions: int32 or int64 (pos_bytes), token n of batch b and axis a at a * pos_axis_stride + b * pos_batch_stride + n.
- * norm: RMS norm in front, over a head (weights [D]) or over the row of all heads (weights [Hq * D] and [Hk * D]), its
- * weights of the type of q and k or 32 bits (weight_dtype); not with `inverse`.  strides, on the host, in elements:
- * (batch, token, head) of q, k, q_out, k_out.  Outputs may be the inputs and overlap them nowhere else.  D and rotary_dim even, rotary_dim <= 512;
- * elements of a head contiguous.  No counterpart in the reference, which leaves positions to its host. */
+ * positions: int32 or int64 (pos_bytes), token n of batch b and axis a at a * pos_axis_stride + b * pos_batch_stride
+ * + n.  norm: RMS norm in front, over a head (weights [D]) or over the row of all heads (weights [Hq * D] and [Hk *
+ * D]), its weights of the type of q and k or 32 bits (weight_dtype); not with `inverse`.  strides, on the host, in
+ * elements: (batch, token, head) of q, k, q_out, k_out.  Outputs may be the inputs and overlap them nowhere else.  D
+ * and rotary_dim even, rotary_dim <= 512; elements of a head contiguous.  No counterpart in the reference, which
+ * leaves positions to its host. */
 int t2t_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight, const void* k_weight,
                int weight_dtype, const void* positions, int pos_bytes, long long pos_axis_stride,
                long long pos_batch_stride, const long long* turns, const int* axis, const long long* strides, int batch,
@@ -337,10 +338,11 @@ int t2t_rotary_grad(const void* dq, const void* dk, const void* q, const void* k
 size_t t2t_fp4_codes_bytes(int M, int K);
 size_t t2t_fp4_scales_bytes(int M, int K, int fmt);
 
-/* Quantises x [M, K].  Scale of a block: T2T_MXFP4 2^(floor(log2 top) - 2), T2T_NVFP4 e4m3(top / 6 / tensor_scale), of its
- * largest magnitude top; codes to the nearest, ties to even, saturating at 6.  A block with a NaN or an infinity becomes
- * NaN.  shift, scale [K] (both or none, of x's type, of 32 bits with dtype + T2T_WIDE_VECTORS): quantises (x - mean) rsqrt(var + eps) (1 + scale) + shift of every
- * row instead.  tensor_scale: 1 for T2T_MXFP4; 2^-100 .. 2^100, and a power of two if ties are to be exact. */
+/* Quantises x [M, K].  Scale of a block: T2T_MXFP4 2^(floor(log2 top) - 2), T2T_NVFP4 e4m3(top / 6 / tensor_scale),
+ * of its largest magnitude top; codes to the nearest, ties to even, saturating at 6.  A block with a NaN or an
+ * infinity becomes NaN.  shift, scale [K] (both or none, of x's type, of 32 bits with dtype + T2T_WIDE_VECTORS):
+ * quantises (x - mean) rsqrt(var + eps) (1 + scale) + shift of every row instead.  tensor_scale: 1 for T2T_MXFP4;
+ * 2^-100 .. 2^100, and a power of two if ties are to be exact. */
 int t2t_fp4_quantize(const void* x, long long x_row_stride, const void* shift, const void* scale, float eps, int M, int K,
                      int dtype, int fmt, float tensor_scale, void* codes, void* scales, cudaStream_t stream);
 
@@ -349,9 +351,10 @@ int t2t_fp4_dequantize(const void* codes, const void* scales, int M, int K, int 
                        long long out_row_stride, int dtype, cudaStream_t stream);
 
 /* out[m, n] = residual[m, n] + gate[n] * act(alpha * sum_k A[m, k] W[n, k] + bias[n]) of 4-bit matrices A [M, K] and
- * W [N, K] of one format; alpha, finite, holds the tensor scales.  Sums in 32 bits, one rounding.  bias, gate [N] (NULL: none) of type
- * vec_dtype, residual [M, N] (NULL: none; row stride 0: one row for all) and out of type dtype; out may be residual (same address and row stride) and overlaps
- * no other input: T2T_ERR_ARG for a factor, not checked for the rest. */
+ * W [N, K] of one format; alpha, finite, holds the tensor scales.  Sums in 32 bits, one rounding.  bias, gate [N]
+ * (NULL: none) of type vec_dtype, residual [M, N] (NULL: none; row stride 0: one row for all) and out of type dtype;
+ * out may be residual (same address and row stride) and overlaps no other input: T2T_ERR_ARG for a factor, not
+ * checked for the rest. */
 int t2t_fp4_matmul(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, int M, int N, int K,
                    int fmt, float alpha, const void* bias, int act, const void* gate, int vec_dtype, const void* residual,
                    long long residual_row_stride, void* out, long long out_row_stride, int dtype, int* d_status,

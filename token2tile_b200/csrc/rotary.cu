@@ -6,7 +6,8 @@
 // on the pairs (2 j, 2 j + 1) or (j, j + rotary_dim / 2) of every head; the rest of the head passes unchanged.  The
 // frequencies come as turns per position in units of 2^-64: the 64-bit product with the position drops whole turns
 // without rounding, so what is off is the position times the error of the frequency itself.  Rotary's, out of 64-bit floats, are right to
-// 2^-55 turns, and the angle to 32 bits up to 2^29 positions (position * f in 32 bits is off by 0.008 rad at 131,072).  Statistics, angles and the rotation are held in 32 bits; each output is rounded once.
+// 2^-55 turns, and the angle to 32 bits up to 2^29 positions (position * f in 32 bits is off by 0.008 rad at 131,072).
+// Statistics, angles and the rotation are held in 32 bits; each output is rounded once.
 //
 // An item is two vectors of V elements that hold V pairs.  L lanes (a power of two) work on one head of one token, a
 // block on all heads of q and k of one token: the cosines are computed once per token and shared by all heads.
@@ -508,8 +509,8 @@ __device__ __forceinline__ void meet(F& v, F* red) {
 // Blocks take tokens in turn, with x of the next two on its way.  One meeting of the block a token: behind it the sums of the norm and
 // the angles of this token (computed one token ahead, in the third of three tables) are there.
 // Bound by memory: q and k of 75,600 tokens of 40 heads of 128, 3.1 GB, take 600 us with the norm over all heads and 530
-// without in a loop over the same tensors (5.2 and 5.8 TB/s), 617 to 639 with the norm where they change from call to call.  One block a token with x loaded to registers took 715; the kernel below, which reads x twice
-// and weights one by one, 1,690.
+// without in a loop over the same tensors (5.2 and 5.8 TB/s), 617 to 639 with the norm where they change from call to call.
+// One block a token with x loaded to registers took 715; the kernel below, which reads x twice and weights one by one, 1,690.
 constexpr int ROT_AHEAD = 3;
 constexpr int fwd_threads(int R) { return R == 4 ? 512 : 256; }
 constexpr int fwd_regs(int R) { return R == 1 ? 104 : 128; }
